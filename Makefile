@@ -3,14 +3,26 @@ HIPCC ?= /opt/rocm/bin/hipcc
 ARCH  ?= gfx950
 LIB   := mfcc_amd/lib/libmfcc_amd.so
 SRC   := mfcc_amd/csrc/mfcc_amd.hip
+SEQ   := mfcc_amd/csrc/sequence_ops.hip
+SEQO  := build/sequence_ops.o
 HDRS  := $(wildcard mfcc_amd/csrc/*.h) include/mfcc_amd.h
-HIPFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -shared -fno-signed-zeros -fno-slp-vectorize -Wall -Wno-unused-function
+HIPFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -fno-signed-zeros -fno-slp-vectorize -Wall -Wno-unused-function
+# the operators along time: no packed float32 instructions (some of their forms have given wrong results on this part)
+SEQFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -c -fno-slp-vectorize -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops
 
 all: $(LIB) host_sim
 
-$(LIB): $(SRC) $(HDRS)
+$(SEQO): $(SEQ) mfcc_amd/csrc/sequence_kernels.h mfcc_amd/csrc/abi.h include/mfcc_amd.h
 	@mkdir -p $(dir $@)
-	$(HIPCC) $(HIPFLAGS) -o $@ $(SRC)
+	$(HIPCC) $(SEQFLAGS) -o $@ $(SEQ)
+
+build/mfcc_amd.o: $(SRC) $(HDRS)
+	@mkdir -p $(dir $@)
+	$(HIPCC) $(HIPFLAGS) -c -o $@ $(SRC)
+
+$(LIB): build/mfcc_amd.o $(SEQO)
+	@mkdir -p $(dir $@)
+	$(HIPCC) --offload-arch=$(ARCH) -fPIC -shared -o $@ $^
 
 host_sim: tests/host_sim/fft_sim
 
@@ -18,16 +30,18 @@ tests/host_sim/fft_sim: tests/host_sim/fft_sim.cpp mfcc_amd/csrc/fft_lane.h mfcc
 	g++ -O2 -std=c++17 -I mfcc_amd/csrc -o $@ $<
 
 # experimental builds for A/B timing: make variant NAME=noslp EXTRA="-fno-slp-vectorize"
-variant: $(SRC) $(HDRS)
+variant: $(SRC) $(HDRS) $(SEQO)
 	@mkdir -p build/variants
-	$(HIPCC) $(HIPFLAGS) $(EXTRA) -o build/variants/libmfcc_$(NAME).so $(SRC)
+	$(HIPCC) $(HIPFLAGS) $(EXTRA) -c -o build/variants/$(NAME).o $(SRC)
+	$(HIPCC) --offload-arch=$(ARCH) -fPIC -shared -o build/variants/libmfcc_$(NAME).so build/variants/$(NAME).o $(SEQO)
 
 # the experimental eight-wave kernel (mfcc_amd/csrc/split_kernel.h) as a library of its own, for
 # tools/split_check.py and tests/test_gpu_split_variant.py
 split: build/variants/libmfcc_split.so
-build/variants/libmfcc_split.so: $(SRC) $(HDRS)
+build/variants/libmfcc_split.so: $(SRC) $(HDRS) $(SEQO)
 	@mkdir -p build/variants
-	$(HIPCC) $(HIPFLAGS) -DMFCC_USE_SPLIT -o $@ $(SRC)
+	$(HIPCC) $(HIPFLAGS) -DMFCC_USE_SPLIT -c -o build/variants/split.o $(SRC)
+	$(HIPCC) --offload-arch=$(ARCH) -fPIC -shared -o $@ build/variants/split.o $(SEQO)
 
 asm: $(SRC) $(HDRS)
 	@mkdir -p build

@@ -268,6 +268,88 @@ int mfcc_utt_scalar_norm(const mfcc_layout* layout, float* feats, int64_t feats_
 int mfcc_pad_batch(const mfcc_layout* layout, const float* feats, int64_t feats_ld, int32_t ncol, int32_t time_steps,
                    float value, int32_t pre_pad, int32_t pre_trunc, float* out, void* stream);
 
+/* ---- operators along time over feature rows: recurrence, running normalisation, dropout ---------
+ * The layers between the rows and the recurrent / CTC consumers.  No counterpart in the reference's
+ * feature path; its recurrent scripts (BiLSTM_7.py, RNN_CTC_17.py) take these inside TensorFlow.
+ *
+ * A batch of sequences is given by three arguments:
+ *   layout, time_steps = 0    rows back to back: sequence u owns the rows [frame_offset[u], frame_offset[u+1])
+ *   layout, time_steps = T    padded batch: sequence u owns the first min(frames[u], T) of its T rows
+ *   layout = NULL             n_seq sequences of T = time_steps rows each
+ * (n_seq is ignored with a layout), and every array of rows by an mfcc_rows: element (sequence u, row t,
+ * column c) sits at data + u * seq_stride + t * row_stride + c, strides in elements, without a
+ * seq_stride at data + (frame_offset[u] + t) * row_stride + c when time_steps = 0.  Inputs may have any
+ * strides >= 0 (row_stride 0: one row for all); rows of outputs must not overlap.  Rows behind the end of a
+ * padded sequence are never read; outputs get 0 there.  Sequences may be empty.  At most 2^31-1 rows per
+ * sequence.  Rows are float32, bfloat16 or float16; states are float32 and the arithmetic is float32. */
+#define MFCC_ROWS_F32 0
+#define MFCC_ROWS_BF16 1
+#define MFCC_ROWS_F16 2
+typedef struct mfcc_rows {
+  void* data;
+  int64_t seq_stride;
+  int64_t row_stride;
+} mfcc_rows;
+
+/* Gated linear recurrence, per sequence and column, h_0 = h0 (float32 [n_seq, ncol], NULL = 0):
+ *   MFCC_SCAN_DECAY    h_t = gate_t h_{t-1} + x_t                 (|gate| <= 1 for a state that stays bounded)
+ *   MFCC_SCAN_SIGMOID  h_t = a_t h_{t-1} + (1 - a_t) x_t,  a_t = 1 / (1 + exp(-gate_t))
+ * y_t = h_t rounded to the type of the rows; last (float32 [n_seq, ncol], may be NULL) = the state behind the
+ * last row, h0 for an empty sequence.  reverse = 1: t runs from the last row of a sequence to its first.
+ * checkpoints: NULL, or mfcc_gated_scan_checkpoints() floats that receive states for the backward pass.
+ * workspace: mfcc_sequence_workspace() bytes of device memory, 16-byte aligned, used by this call only (may be NULL
+ * where that is 0).  y may be x (same strides). */
+#define MFCC_SCAN_DECAY 0
+#define MFCC_SCAN_SIGMOID 1
+int64_t mfcc_gated_scan_checkpoints(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype);
+int64_t mfcc_sequence_workspace(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype);
+int mfcc_gated_scan(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype, int32_t form,
+                    int32_t reverse, const mfcc_rows* x, const mfcc_rows* gate, const float* h0, const mfcc_rows* y, float* last,
+                    float* checkpoints, void* workspace, void* stream);
+/* Gradients of mfcc_gated_scan: from grad_y (rows; NULL = 0) and grad_last (float32 [n_seq, ncol]; NULL = 0) to grad_x,
+ * grad_gate (rows) and grad_h0 (float32 [n_seq, ncol]; may be NULL).  x, gate, h0, checkpoints and the geometry are the
+ * forward call's.  The states are computed again in float32 from the checkpoints, so grad_gate does not suffer from
+ * the rounding of y. */
+int mfcc_gated_scan_backward(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype, int32_t form,
+                             int32_t reverse, const mfcc_rows* x, const mfcc_rows* gate, const float* checkpoints,
+                             const mfcc_rows* grad_y, const float* grad_last, const mfcc_rows* grad_x, const mfcc_rows* grad_gate,
+                             float* grad_h0, void* workspace, void* stream);
+/* One step of the same recurrence for n_seq live sequences: x, gate, y rows [n_seq, ncol] with row strides in
+ * elements, state_in / state_out float32 [n_seq, ncol] contiguous, which may be the same array. */
+int mfcc_gated_scan_step(int64_t n_seq, int32_t ncol, int32_t rows_dtype, int32_t form, const void* x, int64_t x_ld, const void* gate,
+                         int64_t gate_ld, const float* state_in, float* state_out, void* y, int64_t y_ld, void* stream);
+
+/* Running mean / variance normalisation, per sequence and column, causal: with w_0, m_0, s_0 from state_in
+ * (float32 [n_seq, 1 + 2 ncol]: weight, means, weighted sums of squared deviations; NULL = all 0)
+ *   w_t = decay w_{t-1} + 1,  m_t = m_{t-1} + (x_t - m_{t-1}) / w_t,  s_t = decay s_{t-1} + (x_t - m_{t-1})(x_t - m_t)
+ *   y_t = (x_t - m_t) / sqrt(s_t / w_t + eps)            (center_only = 1: y_t = x_t - m_t)
+ * 0 < decay <= 1 (1: cumulative statistics; exact up to 2^24 rows), eps >= 0.  The streaming counterpart of the
+ * corpus constants (x + mm) .* vv (anal_recog_nn_liste.m:180) and of the per-utterance (x - mean) / std
+ * (inference_ctc_eri_05.py:291), which need the whole corpus or utterance.  x is float32; y has y_dtype and may be x
+ * when that is float32 (same strides).  state_out (may be NULL): the state
+ * behind the last row, in an array of its own. */
+int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, double decay, double eps,
+                      int32_t center_only, const mfcc_rows* x, const float* state_in, const mfcc_rows* y, int32_t y_dtype,
+                      float* state_out, void* workspace, void* stream);
+
+/* Dropout whose mask is a function of (seed, step, element number) and is never stored: element e is dropped (y = 0)
+ * when the 16-bit field e mod 8 of the Philox4x32-10 block (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3",
+ * 2011) of counter (e / 8, step) under the key seed is below threshold; kept values are multiplied by 65536 / (65536 -
+ * threshold), so 0 <= threshold <= 65536 is the probability in steps of 2^-16.  With r the row number in the batch
+ * (packed: frame_offset[u] + t, padded: u * time_steps + t) the element number of (u, t, c) is
+ *   MFCC_DROP_ELEMENT   r * ncol + c
+ *   MFCC_DROP_FRAME     r                                   whole rows are dropped
+ *   MFCC_DROP_SEQUENCE  u * ceil(ncol / 8) * 8 + c          a column is dropped for a whole sequence
+ * Applied to a gradient with the same arguments it is the backward pass.  step_device: NULL, or a device int64 that is
+ * read instead of `step` when the kernel runs (for a captured graph whose replays draw new masks).  All rows of a padded
+ * batch are processed.  layout may be NULL with time_steps = rows, n_seq = 1.  y may be x (same strides). */
+#define MFCC_DROP_ELEMENT 0
+#define MFCC_DROP_FRAME 1
+#define MFCC_DROP_SEQUENCE 2
+int mfcc_feature_dropout(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype, int32_t per,
+                         int32_t threshold, uint64_t seed, uint64_t step, const int64_t* step_device, const mfcc_rows* x,
+                         const mfcc_rows* y, void* stream);
+
 /* ---- streaming ------------------------------------------------------------------------
  * n_streams live streams that advance in lock step (every push brings the same number of
  * samples for each).  The reference has no incremental routine -- its live script queues

@@ -19,4 +19,6 @@ __all__ = [
 ]
 from . import cnn, corpus, datasets, psf, sequences  # noqa: E402,F401  (counterparts of the reference's data plumbing / call sites)
 from .corpus import corpus_mfcc_cmvn  # noqa: E402,F401
+from .recurrent import (feature_dropout, gated_scan, gated_scan_step, running_norm,  # noqa: E402,F401
+                        running_norm_state)
 from .sequences import ctc_feature_batch, pad_sequences, utterance_scalar_norm  # noqa: E402,F401

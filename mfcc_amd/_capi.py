@@ -21,6 +21,9 @@ OUT_MFCC39, OUT_STATIC, OUT_LOGMEL, OUT_SPEC, OUT_LOGSPEC = 0, 1, 2, 3, 4
 STACK_FRAME_MAJOR, STACK_TILE = 0, 1
 KERNEL_AUTO, KERNEL_GENERAL = 0, 1
 CMVN_STATIC_MAX_COLS = 264
+ROWS_F32, ROWS_BF16, ROWS_F16 = 0, 1, 2
+SCAN_DECAY, SCAN_SIGMOID = 0, 1
+DROP_ELEMENT, DROP_FRAME, DROP_SEQUENCE = 0, 1, 2
 
 
 class MfccConfig(C.Structure):
@@ -47,6 +50,11 @@ class MfccConfig(C.Structure):
     ]
 
 
+class MfccRows(C.Structure):
+    """struct mfcc_rows: one array of rows, strides in elements"""
+    _fields_ = [("data", C.c_void_p), ("seq_stride", C.c_int64), ("row_stride", C.c_int64)]
+
+
 class MfccError(RuntimeError):
     def __init__(self, code, msg):
         super().__init__(f"libmfcc_amd error {code}: {msg}")
@@ -54,6 +62,8 @@ class MfccError(RuntimeError):
 
 
 _vp, _i32, _i64, _dbl = C.c_void_p, C.c_int32, C.c_int64, C.c_double
+_u64, _rowsp = C.c_uint64, C.POINTER(MfccRows)
+_seqs = [_vp, _i64, _i64, _i32]   # layout, n_seq, time_steps, ncol
 _i32p, _i64p, _dblp = C.POINTER(C.c_int32), C.POINTER(C.c_int64), C.POINTER(C.c_double)
 
 # name -> (restype, argtypes); every symbol declared in include/mfcc_amd.h
@@ -94,6 +104,13 @@ SIGNATURES = {
     "mfcc_cmvn_apply": (C.c_int, [_vp, _i64, _i64, _i32, _vp, _vp, _vp]),
     "mfcc_utt_scalar_norm": (C.c_int, [_vp, _vp, _i64, _i32, _vp]),
     "mfcc_pad_batch": (C.c_int, [_vp, _vp, _i64, _i32, _i32, C.c_float, _i32, _i32, _vp, _vp]),
+    "mfcc_gated_scan_checkpoints": (_i64, _seqs + [_i32]),
+    "mfcc_sequence_workspace": (_i64, _seqs + [_i32]),
+    "mfcc_gated_scan": (C.c_int, _seqs + [_i32, _i32, _i32, _rowsp, _rowsp, _vp, _rowsp, _vp, _vp, _vp, _vp]),
+    "mfcc_gated_scan_backward": (C.c_int, _seqs + [_i32, _i32, _i32, _rowsp, _rowsp, _vp, _rowsp, _vp, _rowsp, _rowsp, _vp, _vp, _vp]),
+    "mfcc_gated_scan_step": (C.c_int, [_i64, _i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp]),
+    "mfcc_running_norm": (C.c_int, _seqs + [_dbl, _dbl, _i32, _rowsp, _vp, _rowsp, _i32, _vp, _vp, _vp]),
+    "mfcc_feature_dropout": (C.c_int, _seqs + [_i32, _i32, _i32, _u64, _u64, _vp, _rowsp, _rowsp, _vp]),
     "mfcc_stream_create": (C.c_int, [_vp, _i32, _i32, _i32, C.POINTER(_vp)]),
     "mfcc_stream_destroy": (C.c_int, [_vp]),
     "mfcc_stream_reset": (C.c_int, [_vp]),

@@ -13,6 +13,7 @@
 #include <numeric>
 #include <vector>
 
+#include "abi.h"
 #include "fused_kernel.h"
 #include "general_kernel.h"
 #ifdef MFCC_USE_SPLIT  // experimental build: MFCC-39 through the eight-wave kernel of split_kernel.h
@@ -26,7 +27,9 @@ namespace {
 
 thread_local char g_err[512] = "";
 
-int fail(int code, const char* fmt, ...) {
+}  // namespace
+
+int mfcc::fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_err, sizeof(g_err), fmt, ap);
@@ -34,11 +37,9 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-#define HIP_TRY(expr)                                                                        \
-  do {                                                                                       \
-    hipError_t e_ = (expr);                                                                  \
-    if (e_ != hipSuccess) return fail(MFCC_ERR_HIP, "%s: %s", #expr, hipGetErrorString(e_)); \
-  } while (0)
+using mfcc::fail;
+
+namespace {
 
 template <typename T>
 int upload(const std::vector<T>& host, T** dev) {
@@ -48,8 +49,6 @@ int upload(const std::vector<T>& host, T** dev) {
   HIP_TRY(hipMemcpy(*dev, host.data(), host.size() * sizeof(T), hipMemcpyHostToDevice));
   return MFCC_OK;
 }
-
-inline unsigned blocks_for(int64_t n, int per) { return (unsigned)((n + per - 1) / per); }
 
 // Partial sums of mfcc_cmvn_accumulate: one buffer per (device, stream) that has called it, sized
 // at its first call for the widest rows the entry point takes (so it is never grown, freed or
@@ -182,27 +181,6 @@ struct mfcc_plan {
   int32_t* g_band = nullptr;
   float* g_dctl = nullptr;
   float* g_window = nullptr;
-};
-
-struct mfcc_layout {
-  int device;
-  int64_t n_utts, total_samples, total_frames;
-  std::vector<int64_t> sample_off, frame_off;
-  int64_t* d_sample_off = nullptr;
-  int64_t* d_frame_off = nullptr;
-  mfcc::Tile* d_tiles = nullptr;
-  int64_t n_tiles;
-  // the same frames cut for the persistent workgroups of split_kernel.h: workgroup w walks
-  // d_wg_tiles[d_wg_off[w] .. d_wg_off[w + 1]); every workgroup gets about the same number of batches
-  mfcc::Tile* d_wg_tiles = nullptr;
-  int32_t* d_wg_off = nullptr;
-  int32_t n_wg = 0;
-  bool frames_only = false;  // made by mfcc_layout_create_frames: frame offsets only, no audio geometry
-  // what the tile list was cut for: a plan may only run on a layout of its own framing whose
-  // tiles fit its kernel
-  int32_t frame_size = 0, frame_step = 0, frame_rule = 0;
-  int32_t max_nt = 0;  // most output frames in one tile
-  bool general_cut = false;  // tiles cut for the general kernel (no halo rule)
 };
 
 struct mfcc_stream {
@@ -408,7 +386,7 @@ static int layout_fits(const mfcc_plan* plan, const mfcc_layout* layout) {
 
 extern "C" {
 
-int mfcc_version(void) { return 101; }
+int mfcc_version(void) { return 102; }
 
 const char* mfcc_last_error(void) { return g_err; }
 
@@ -922,6 +900,7 @@ static int layout_create_impl(const mfcc_plan* plan, const int64_t* lengths_host
     }
     l->sample_off[u + 1] = l->sample_off[u] + len;
     l->frame_off[u + 1] = l->frame_off[u] + nf;
+    l->longest = std::max(l->longest, (int64_t)nf);
     // greedy tiling: every tile computes a whole number of 16-frame batches where it can
     // (tile frames + 4 halo frames on each side that continues)
     for (int64_t t = 0; t < nf;) {
@@ -1026,6 +1005,7 @@ int mfcc_layout_create_frames(int device, const int64_t* frame_counts_host, int6
         return fail(MFCC_ERR_INVALID, "utterance %lld has a negative frame count", (long long)u);
       }
       l->frame_off[u + 1] = l->frame_off[u] + frame_counts_host[u];
+      l->longest = std::max(l->longest, frame_counts_host[u]);
     }
     l->total_samples = 0;
     l->total_frames = l->frame_off[n_utts];

@@ -1,0 +1,219 @@
+// C entry points of the operators along time (see "operators along time over feature rows" in include/mfcc_amd.h).
+#include <algorithm>
+
+#include "abi.h"
+#include "sequence_kernels.h"
+
+using mfcc::Batch;
+using mfcc::fail;
+using mfcc::Rows;
+
+namespace {
+
+constexpr int64_t kMaxColumns = 1 << 20;
+
+// The geometry of a call, checked once: 0 or a negative error code.
+struct Shape {
+  Batch b;
+  int64_t longest, rows;  // most rows of one sequence; rows of all of them, padding included
+};
+int shape_of(const char* who, const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t reverse, Shape* out) {
+  if (ncol < 1 || ncol > kMaxColumns) return fail(MFCC_ERR_INVALID, "%s: ncol=%d outside 1..%lld", who, ncol, (long long)kMaxColumns);
+  if (time_steps < 0 || time_steps > INT32_MAX) return fail(MFCC_ERR_INVALID, "%s: time_steps=%lld outside 0..2^31-1", who, (long long)time_steps);
+  if (layout) n_seq = layout->n_utts;
+  if (n_seq < 0 || n_seq > INT32_MAX) return fail(MFCC_ERR_INVALID, "%s: %lld sequences outside 0..2^31-1", who, (long long)n_seq);
+  out->b = Batch{layout ? layout->d_frame_off : nullptr, n_seq, time_steps, ncol, reverse};
+  out->longest = layout ? (time_steps ? std::min(layout->longest, time_steps) : layout->longest) : time_steps;
+  out->rows = time_steps || !layout ? n_seq * time_steps : layout->total_frames;
+  if (out->longest > INT32_MAX) return fail(MFCC_ERR_UNSUPPORTED, "%s: a sequence of more than 2^31-1 rows", who);
+  if (!layout && time_steps == 0) out->b.n_seq = n_seq;  // sequences without rows: states pass through
+  return MFCC_OK;
+}
+
+int check_rows(const char* who, const char* name, const mfcc_rows* r, const Shape& s, bool output) {
+  if (!r || (!r->data && s.rows > 0)) return fail(MFCC_ERR_INVALID, "%s: %s is null", who, name);
+  if (r->row_stride < 0 || r->seq_stride < 0) return fail(MFCC_ERR_INVALID, "%s: negative stride of %s", who, name);
+  if (output && s.rows > 1) {
+    // rows of outputs do not overlap: one row after the other inside a sequence and sequence after sequence, or
+    // time-major (all sequences' row t, then row t + 1)
+    const int64_t nc = s.b.ncol, rs = r->row_stride, ss = r->seq_stride, n = s.b.n_seq, t = s.b.steps;
+    const bool packed = t == 0;
+    const bool ok = packed ? rs >= nc
+                           : ((t == 1 || rs >= nc) && (n == 1 || ss >= (t - 1) * rs + nc)) || ((n == 1 || ss >= nc) && (t == 1 || rs >= (n - 1) * ss + nc));
+    if (!ok) return fail(MFCC_ERR_INVALID, "%s: rows of %s overlap (row stride %lld, sequence stride %lld, %lld columns)", who, name,
+                         (long long)rs, (long long)ss, (long long)nc);
+  }
+  return MFCC_OK;
+}
+
+template <typename T>
+Rows<T> rows_of(const mfcc_rows* r) {
+  return r ? Rows<T>{(T*)r->data, r->seq_stride, r->row_stride} : Rows<T>{nullptr, 0, 0};
+}
+
+int bad_dtype(const char* who, int32_t dtype) { return fail(MFCC_ERR_INVALID, "%s: rows type %d", who, dtype); }
+
+}  // namespace
+
+extern "C" {
+
+int64_t mfcc_gated_scan_checkpoints(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype) {
+  Shape s;
+  if (const int rc = shape_of("mfcc_gated_scan_checkpoints", layout, n_seq, time_steps, ncol, 0, &s)) return rc;
+  if (rows_dtype < 0 || rows_dtype > MFCC_ROWS_F16) return bad_dtype("mfcc_gated_scan_checkpoints", rows_dtype);
+  const int64_t k = mfcc::kScanTile;
+  return (time_steps || !layout ? s.b.n_seq * ((time_steps + k - 1) / k) : s.rows / k + s.b.n_seq) * ncol;
+}
+
+int64_t mfcc_sequence_workspace(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype) {
+  Shape s;
+  if (const int rc = shape_of("mfcc_sequence_workspace", layout, n_seq, time_steps, ncol, 0, &s)) return rc;
+  if (rows_dtype < 0 || rows_dtype > MFCC_ROWS_F16) return bad_dtype("mfcc_sequence_workspace", rows_dtype);
+  return 0;
+}
+
+int mfcc_gated_scan(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype, int32_t form,
+                    int32_t reverse, const mfcc_rows* x, const mfcc_rows* gate, const float* h0, const mfcc_rows* y, float* last,
+                    float* checkpoints, void* workspace, void* stream) {
+  static const char who[] = "mfcc_gated_scan";
+  Shape s;
+  if (const int rc = shape_of(who, layout, n_seq, time_steps, ncol, reverse ? 1 : 0, &s)) return rc;
+  if (form != MFCC_SCAN_DECAY && form != MFCC_SCAN_SIGMOID) return fail(MFCC_ERR_INVALID, "%s: form=%d", who, form);
+  if (const int rc = check_rows(who, "x", x, s, false)) return rc;
+  if (const int rc = check_rows(who, "gate", gate, s, false)) return rc;
+  if (const int rc = check_rows(who, "y", y, s, true)) return rc;
+  const int64_t total = s.b.n_seq * ncol;
+  if (total == 0) return MFCC_OK;
+  const mfcc::ScanPtrs q{h0, nullptr, last, checkpoints, nullptr};
+  auto go = [&](auto zero) {
+    using T = decltype(zero);
+    auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_kernel<T, true> : mfcc::gated_scan_kernel<T, false>;
+    hipLaunchKernelGGL(k, dim3(blocks_for(total, 256)), dim3(256), 0, (hipStream_t)stream, s.b, rows_of<const T>(x), rows_of<const T>(gate),
+                       rows_of<T>(y), q);
+  };
+  switch (rows_dtype) {
+    case MFCC_ROWS_F32: go(0.0f); break;
+    case MFCC_ROWS_BF16: go((mfcc::bf16)0.0f); break;
+    case MFCC_ROWS_F16: go((mfcc::f16)0.0f); break;
+    default: return bad_dtype(who, rows_dtype);
+  }
+  HIP_TRY(hipGetLastError());
+  return MFCC_OK;
+}
+
+int mfcc_gated_scan_backward(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype, int32_t form,
+                             int32_t reverse, const mfcc_rows* x, const mfcc_rows* gate, const float* checkpoints,
+                             const mfcc_rows* grad_y, const float* grad_last, const mfcc_rows* grad_x, const mfcc_rows* grad_gate,
+                             float* grad_h0, void* workspace, void* stream) {
+  static const char who[] = "mfcc_gated_scan_backward";
+  Shape s;
+  if (const int rc = shape_of(who, layout, n_seq, time_steps, ncol, reverse ? 1 : 0, &s)) return rc;
+  if (form != MFCC_SCAN_DECAY && form != MFCC_SCAN_SIGMOID) return fail(MFCC_ERR_INVALID, "%s: form=%d", who, form);
+  if (const int rc = check_rows(who, "x", x, s, false)) return rc;
+  if (const int rc = check_rows(who, "gate", gate, s, false)) return rc;
+  if (grad_y)
+    if (const int rc = check_rows(who, "grad_y", grad_y, s, false)) return rc;
+  if (const int rc = check_rows(who, "grad_x", grad_x, s, true)) return rc;
+  if (const int rc = check_rows(who, "grad_gate", grad_gate, s, true)) return rc;
+  if (!checkpoints && s.rows > 0) return fail(MFCC_ERR_INVALID, "%s: checkpoints is null", who);
+  const int64_t total = s.b.n_seq * ncol;
+  if (total == 0) return MFCC_OK;
+  const mfcc::ScanPtrs q{nullptr, grad_last, nullptr, const_cast<float*>(checkpoints), grad_h0};
+  auto go = [&](auto zero) {
+    using T = decltype(zero);
+    auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_backward_kernel<T, true> : mfcc::gated_scan_backward_kernel<T, false>;
+    hipLaunchKernelGGL(k, dim3(blocks_for(total, 256)), dim3(256), 0, (hipStream_t)stream, s.b, rows_of<const T>(x), rows_of<const T>(gate),
+                       rows_of<const T>(grad_y), rows_of<T>(grad_x), rows_of<T>(grad_gate), q);
+  };
+  switch (rows_dtype) {
+    case MFCC_ROWS_F32: go(0.0f); break;
+    case MFCC_ROWS_BF16: go((mfcc::bf16)0.0f); break;
+    case MFCC_ROWS_F16: go((mfcc::f16)0.0f); break;
+    default: return bad_dtype(who, rows_dtype);
+  }
+  HIP_TRY(hipGetLastError());
+  return MFCC_OK;
+}
+
+int mfcc_gated_scan_step(int64_t n_seq, int32_t ncol, int32_t rows_dtype, int32_t form, const void* x, int64_t x_ld, const void* gate,
+                         int64_t gate_ld, const float* state_in, float* state_out, void* y, int64_t y_ld, void* stream) {
+  static const char who[] = "mfcc_gated_scan_step";
+  if (ncol < 1 || ncol > kMaxColumns || n_seq < 0 || n_seq > INT32_MAX || x_ld < 0 || gate_ld < 0) return fail(MFCC_ERR_INVALID, "%s: bad shape", who);
+  if (n_seq > 1 && y_ld < ncol) return fail(MFCC_ERR_INVALID, "%s: rows of y overlap", who);
+  if (form != MFCC_SCAN_DECAY && form != MFCC_SCAN_SIGMOID) return fail(MFCC_ERR_INVALID, "%s: form=%d", who, form);
+  if (n_seq == 0) return MFCC_OK;
+  if (!x || !gate || !state_in || !state_out || !y) return fail(MFCC_ERR_INVALID, "%s: null pointer", who);
+  auto go = [&](auto zero) {
+    using T = decltype(zero);
+    auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_step_kernel<T, true> : mfcc::gated_scan_step_kernel<T, false>;
+    hipLaunchKernelGGL(k, dim3(blocks_for(n_seq * ncol, 256)), dim3(256), 0, (hipStream_t)stream, n_seq, ncol, (const T*)x, x_ld,
+                       (const T*)gate, gate_ld, state_in, state_out, (T*)y, y_ld);
+  };
+  switch (rows_dtype) {
+    case MFCC_ROWS_F32: go(0.0f); break;
+    case MFCC_ROWS_BF16: go((mfcc::bf16)0.0f); break;
+    case MFCC_ROWS_F16: go((mfcc::f16)0.0f); break;
+    default: return bad_dtype(who, rows_dtype);
+  }
+  HIP_TRY(hipGetLastError());
+  return MFCC_OK;
+}
+
+int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, double decay, double eps,
+                      int32_t center_only, const mfcc_rows* x, const float* state_in, const mfcc_rows* y, int32_t y_dtype,
+                      float* state_out, void* workspace, void* stream) {
+  static const char who[] = "mfcc_running_norm";
+  Shape s;
+  if (const int rc = shape_of(who, layout, n_seq, time_steps, ncol, 0, &s)) return rc;
+  if (!(decay > 0.0 && decay <= 1.0)) return fail(MFCC_ERR_INVALID, "%s: decay=%g outside (0, 1]", who, decay);
+  if (!(eps >= 0.0 && eps <= 1e30)) return fail(MFCC_ERR_INVALID, "%s: eps=%g", who, eps);
+  if (const int rc = check_rows(who, "x", x, s, false)) return rc;
+  if (const int rc = check_rows(who, "y", y, s, true)) return rc;
+  if (state_in && state_in == state_out) return fail(MFCC_ERR_INVALID, "%s: state_out needs an array of its own", who);
+  const int64_t total = s.b.n_seq * ncol;
+  if (total == 0) return MFCC_OK;
+  auto go = [&](auto zero) {
+    using T = decltype(zero);
+    hipLaunchKernelGGL(mfcc::running_norm_kernel<T>, dim3(blocks_for(total, 256)), dim3(256), 0, (hipStream_t)stream, s.b,
+                       rows_of<const float>(x), rows_of<T>(y), decay, (float)eps, center_only ? 1 : 0, state_in, state_out);
+  };
+  switch (y_dtype) {
+    case MFCC_ROWS_F32: go(0.0f); break;
+    case MFCC_ROWS_BF16: go((mfcc::bf16)0.0f); break;
+    case MFCC_ROWS_F16: go((mfcc::f16)0.0f); break;
+    default: return bad_dtype(who, y_dtype);
+  }
+  HIP_TRY(hipGetLastError());
+  return MFCC_OK;
+}
+
+int mfcc_feature_dropout(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype, int32_t per,
+                         int32_t threshold, uint64_t seed, uint64_t step, const int64_t* step_device, const mfcc_rows* x,
+                         const mfcc_rows* y, void* stream) {
+  static const char who[] = "mfcc_feature_dropout";
+  Shape s;
+  if (const int rc = shape_of(who, layout, n_seq, time_steps, ncol, 0, &s)) return rc;
+  if (per < MFCC_DROP_ELEMENT || per > MFCC_DROP_SEQUENCE) return fail(MFCC_ERR_INVALID, "%s: per=%d", who, per);
+  if (threshold < 0 || threshold > 65536) return fail(MFCC_ERR_INVALID, "%s: threshold=%d outside 0..65536", who, threshold);
+  if (const int rc = check_rows(who, "x", x, s, false)) return rc;
+  if (const int rc = check_rows(who, "y", y, s, true)) return rc;
+  if (s.rows == 0) return MFCC_OK;
+  const float scale = threshold < 65536 ? 65536.0f / (float)(65536 - threshold) : 0.0f;
+  const int64_t total = s.rows * ncol;
+  if ((total + 255) / 256 > INT32_MAX) return fail(MFCC_ERR_UNSUPPORTED, "%s: too many rows per call", who);
+  auto go = [&](auto zero) {
+    using T = decltype(zero);
+    hipLaunchKernelGGL(mfcc::feature_dropout_kernel<T>, dim3(blocks_for(total, 256)), dim3(256), 0, (hipStream_t)stream, s.b, s.rows, per,
+                       (uint32_t)threshold, scale, seed, step, step_device, rows_of<const T>(x), rows_of<T>(y));
+  };
+  switch (rows_dtype) {
+    case MFCC_ROWS_F32: go(0.0f); break;
+    case MFCC_ROWS_BF16: go((mfcc::bf16)0.0f); break;
+    case MFCC_ROWS_F16: go((mfcc::f16)0.0f); break;
+    default: return bad_dtype(who, rows_dtype);
+  }
+  HIP_TRY(hipGetLastError());
+  return MFCC_OK;
+}
+
+}  // extern "C"

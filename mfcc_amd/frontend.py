@@ -518,9 +518,18 @@ class StreamingMFCC:
     [n_streams, k, 39]; a row is final once the 4 frames after it are complete.  ``flush()``
     returns the remaining rows (zero-padded last frame, edge-replicated deltas) and starts a new
     utterance.  All rows of one utterance, concatenated, equal the whole-utterance result
-    (main(), mfcc-self5.py:211-229) on the concatenated audio."""
+    (main(), mfcc-self5.py:211-229) on the concatenated audio.
 
-    def __init__(self, variant="self5", n_streams=1, max_chunk=1600, dtype=torch.int16, device=None, **overrides):
+    ``running_norm=decay`` returns the rows normalised by their running mean and variance
+    (:func:`~mfcc_amd.running_norm`, one more launch a push): every utterance starts from ``norm_state``
+    (float32 [n_streams or 1, 1 + 2*39], e.g. running_norm_state of corpus sums; default no prior)."""
+
+    def __init__(self, variant="self5", n_streams=1, max_chunk=1600, dtype=torch.int16, device=None, running_norm=None, norm_state=None,
+                 **overrides):
+        if running_norm is None and norm_state is not None:
+            raise ValueError("norm_state is the prior of running_norm")
+        if running_norm is not None and not 0.0 < running_norm <= 1.0:
+            raise ValueError("running_norm must be a decay in (0, 1]")
         if dtype not in (torch.int16, torch.float32):
             raise ValueError("dtype must be torch.int16 or torch.float32")
         cfg = dict(VARIANTS[variant])
@@ -534,6 +543,24 @@ class StreamingMFCC:
                                                       C.byref(self._h)))
         self.max_rows = capi.load().mfcc_stream_max_rows(self._h)
         self.width = self.plan.out_width("mfcc39")
+        self._decay = running_norm
+        if running_norm is not None:
+            shape = (self.n_streams, 1 + 2 * self.width)
+            prior = torch.zeros(shape, dtype=torch.float32, device=self.plan.device)
+            if norm_state is not None:
+                prior.copy_(norm_state.expand(shape))
+            # the state before a push and behind it take turns: a push reads one array and writes the other
+            self._prior, self._norm = prior, [torch.empty_like(prior), torch.empty_like(prior)]
+            self._state = prior
+
+    def _normed(self, rows):
+        """The rows of one push, [n_streams, k, width], normalised in place; the state moves on."""
+        if self._decay is not None and rows.shape[1]:
+            from .recurrent import running_norm
+            into = self._norm[1] if self._state is self._norm[0] else self._norm[0]
+            running_norm(rows, decay=self._decay, state=self._state, out=rows, state_out=into)
+            self._state = into
+        return rows
 
     def _out(self):
         return torch.empty((self.n_streams, self.max_rows, self.width), dtype=torch.float32, device=self.plan.device)
@@ -558,7 +585,7 @@ class StreamingMFCC:
             ld = max(t.stride(0), t.shape[1]) if self.n_streams == 1 else t.stride(0)
             capi.check(capi.load().mfcc_stream_push(self._h, _ptr(t), ld, t.shape[1],
                                                     _ptr(out), out.stride(0), out.stride(1), C.byref(k), _stream_ptr()))
-        return _ret(out[:, :k.value], was_numpy)
+        return _ret(self._normed(out[:, :k.value, :self.width]) if self._decay is not None else out[:, :k.value], was_numpy)
 
     def flush(self, out=None, as_numpy=False):
         if out is None:
@@ -567,10 +594,16 @@ class StreamingMFCC:
         with _on(self.plan.device, out):
             capi.check(capi.load().mfcc_stream_flush(self._h, _ptr(out), out.stride(0), out.stride(1), C.byref(k),
                                                      _stream_ptr()))
-        return _ret(out[:, :k.value], as_numpy)
+        rows = out[:, :k.value]
+        if self._decay is not None:
+            rows = self._normed(rows[..., :self.width])
+            self._state = self._prior    # the next push starts new utterances
+        return _ret(rows, as_numpy)
 
     def reset(self):
         capi.check(capi.load().mfcc_stream_reset(self._h))
+        if self._decay is not None:
+            self._state = self._prior
 
     def __del__(self):
         h, self._h = getattr(self, "_h", None), None

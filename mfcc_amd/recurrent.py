@@ -1,0 +1,346 @@
+"""Operators along time over feature rows, on the device: the gated linear recurrence with its
+gradient and its single-step form, the running (causal) mean / variance normalisation of live rows,
+and the dropout whose mask is a function of a counter and is never stored.
+
+They stand between the rows of the front-end and its recurrent / CTC consumers (BiLSTM_7.py,
+RNN_CTC_17.py), and take the batches that the rest of the package makes: packed rows ``[sum F, D]``
+with frame counts (``MFCC.forward``), or a padded ``[B, T, D]`` batch with lengths (``pad_sequences``,
+'post' padding).  ``frame_counts`` is a sequence of counts, a :class:`~mfcc_amd.Layout` (keep one for
+repeated batch shapes; required while a stream is being captured) or None: all rows are one sequence
+(2-D) or every sequence is full (3-D).  Lengths beyond T count as T, as ``pad_sequences`` reports
+them.  Rows behind the end of a padded sequence are not read; outputs hold 0 there.
+"""
+from __future__ import annotations
+
+import numpy as np
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _capi as capi
+from .frontend import Layout, _on, frames_layout
+
+_ROWS = {torch.float32: capi.ROWS_F32, torch.bfloat16: capi.ROWS_BF16, torch.float16: capi.ROWS_F16}
+_FORMS = {"decay": capi.SCAN_DECAY, "sigmoid": capi.SCAN_SIGMOID}
+_PER = {"element": capi.DROP_ELEMENT, "frame": capi.DROP_FRAME, "sequence": capi.DROP_SEQUENCE}
+
+
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+class _Batch:
+    """Geometry of one call: the layout handle, the number of sequences, the padded length (0 = packed)."""
+    __slots__ = ("layout", "handle", "n_seq", "steps", "ncol")
+
+    def __init__(self, x, frame_counts):
+        if x.dim() not in (2, 3):
+            raise ValueError("rows must be [rows, D] or [B, T, D]")
+        self.ncol = x.shape[-1]
+        if self.ncol < 1:
+            raise ValueError("rows without columns")
+        self.layout = None
+        if frame_counts is not None:
+            if not isinstance(frame_counts, Layout):
+                if torch.cuda.is_current_stream_capturing():
+                    raise ValueError("while a stream is captured, pass a Layout that outlives the graph instead of frame counts")
+                if isinstance(frame_counts, torch.Tensor):
+                    frame_counts = frame_counts.cpu().numpy()
+                frame_counts = np.asarray(frame_counts, dtype=np.int64).reshape(-1)
+                if len(frame_counts) and frame_counts.min() < 0:
+                    raise ValueError("negative frame count")
+                self._fits(x, len(frame_counts), int(frame_counts.sum()))
+                frame_counts = frames_layout(x.device, frame_counts)
+            else:
+                self._fits(x, frame_counts.n_utts, frame_counts.total_frames)
+            if frame_counts.device != x.device:
+                raise ValueError(f"layout on {frame_counts.device}, rows on {x.device}")
+            self.layout = frame_counts
+        if x.dim() == 2:
+            self.n_seq = 1 if self.layout is None else self.layout.n_utts
+            self.steps = x.shape[0] if self.layout is None else 0
+        else:
+            self.n_seq, self.steps = x.shape[0], x.shape[1]
+            if self.steps == 0:
+                self.layout = None    # no rows at all, whatever the lengths say
+        self.handle = None if self.layout is None else self.layout._h
+
+    @staticmethod
+    def _fits(x, n_seq, total):
+        if x.dim() == 2 and total != x.shape[0]:
+            raise ValueError("frame_counts do not add up to the number of rows")
+        if x.dim() == 3 and n_seq != x.shape[0]:
+            raise ValueError(f"{n_seq} lengths for a batch of {x.shape[0]}")
+
+    def head(self):
+        return self.handle, self.n_seq, self.steps, self.ncol
+
+
+def _rows(t):
+    if t.dim() == 3:
+        return capi.MfccRows(t.data_ptr(), t.stride(0), t.stride(1))
+    return capi.MfccRows(t.data_ptr(), 0, t.stride(0))
+
+
+def _check(t, name, like=None, dtypes=_ROWS):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise ValueError(f"{name} must be a device tensor of " + " / ".join(str(d).replace("torch.", "") for d in dtypes)
+                         + " with unit column stride")
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype):
+        raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype}, expected {tuple(like.shape)} {like.dtype}")
+    return t
+
+
+def _check_state(t, name, shape):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32 or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be a float32 device tensor {tuple(shape)}")
+    return t
+
+
+def _out(out, shape, dtype, device):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if (not isinstance(out, torch.Tensor) or tuple(out.shape) != tuple(shape) or out.dtype != dtype or not out.is_cuda
+            or (out.stride(-1) != 1 and shape[-1] > 1)):
+        raise ValueError(f"out must be a {dtype} device tensor {tuple(shape)} with unit column stride")
+    if out.requires_grad:
+        raise ValueError("out requires a gradient")
+    return out
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _workspace(batch, dtype, device):
+    n = capi.check(capi.load().mfcc_sequence_workspace(*batch.head(), _ROWS[dtype]))
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def _no_grad(*tensors):
+    return not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
+
+
+# --------------------------------------------------------------------------
+# gated linear recurrence
+# --------------------------------------------------------------------------
+def _scan_forward(x, gate, h0, batch, form, reverse, out, keep):
+    lib = capi.load()
+    y = _out(out, x.shape, x.dtype, x.device)
+    last = torch.empty((batch.n_seq, batch.ncol), dtype=torch.float32, device=x.device)
+    code = _ROWS[x.dtype]
+    with _on(x.device, gate, h0, y):
+        ckpt = None
+        if keep:
+            ckpt = torch.empty(capi.check(lib.mfcc_gated_scan_checkpoints(*batch.head(), code)), dtype=torch.float32, device=x.device)
+        ws = _workspace(batch, x.dtype, x.device)
+        capi.check(lib.mfcc_gated_scan(*batch.head(), code, form, reverse, _rows(x), _rows(gate), _ptr(h0), _rows(y), last.data_ptr(),
+                                       _ptr(ckpt), _ptr(ws), _stream()))
+    return y, last, ckpt
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, h0, batch, form, reverse):
+        y, last, ckpt = _scan_forward(x, gate, h0, batch, form, reverse, None, True)
+        ctx.save_for_backward(x, gate, ckpt)
+        ctx.geometry = batch, form, reverse
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, glast):
+        x, gate, ckpt = ctx.saved_tensors
+        batch, form, reverse = ctx.geometry
+        if gy is None and glast is None:
+            return (None,) * 6
+        if gy is not None and gy.stride(-1) != 1 and gy.shape[-1] > 1:
+            gy = gy.contiguous()
+        if glast is not None:
+            glast = glast.contiguous()
+        gx, gg = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        gh0 = torch.empty((batch.n_seq, batch.ncol), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
+        with _on(x.device, gy, glast):
+            ws = _workspace(batch, x.dtype, x.device)
+            capi.check(capi.load().mfcc_gated_scan_backward(
+                *batch.head(), _ROWS[x.dtype], form, reverse, _rows(x), _rows(gate), ckpt.data_ptr(), None if gy is None else _rows(gy),
+                _ptr(glast), _rows(gx), _rows(gg), _ptr(gh0), _ptr(ws), _stream()))
+        need = ctx.needs_input_grad
+        return gx if need[0] else None, gg if need[1] else None, gh0, None, None, None
+
+
+def gated_scan(x, gate, frame_counts=None, h0=None, form="decay", reverse=False, out=None):
+    """The recurrence of a gated linear layer along time, per sequence and column, from ``h0``
+    (float32 [n_seq, D], default 0):
+
+    ``form='decay'``    h_t = gate_t h_{t-1} + x_t          (gates are decays: abs(gate) <= 1)
+    ``form='sigmoid'``  h_t = a_t h_{t-1} + (1 - a_t) x_t,  a_t = 1 / (1 + exp(-gate_t))
+
+    ``x`` and ``gate`` are float32, bfloat16 or float16 rows of one shape (any row strides; an expanded
+    ``gate[D]`` is one gate for all rows); ``reverse`` runs each sequence from its last row to its first,
+    the other half of a bidirectional layer.  Returns (y, last): y_t = h_t in the type of ``x``, and the
+    float32 state behind the last row [n_seq, D] (``h0`` where a sequence is empty), which is the ``h0``
+    of the next piece.  The state is float32 throughout.  Differentiable in x, gate and h0 (once): the
+    backward pass computes the states again from float32 checkpoints instead of reading the rounded y.
+    ``out`` takes y when no gradient is asked for; it may be ``x``."""
+    _check(x, "x")
+    _check(gate, "gate", like=x)
+    if form not in _FORMS:
+        raise ValueError("form must be 'decay' or 'sigmoid'")
+    batch = _Batch(x, frame_counts)
+    h0 = _check_state(h0, "h0", (batch.n_seq, batch.ncol))
+    if h0 is not None:
+        h0 = h0.contiguous()
+    if _no_grad(x, gate, h0):
+        return _scan_forward(x, gate, h0, batch, _FORMS[form], int(bool(reverse)), out, False)[:2]
+    if out is not None:
+        raise ValueError("out is for calls without gradients")
+    return _GatedScan.apply(x, gate, h0, batch, _FORMS[form], int(bool(reverse)))
+
+
+def gated_scan_step(x, gate, state, form="decay", out=None, state_out=None):
+    """One step of :func:`gated_scan` for live sequences that advance in lock step: x, gate [n_seq, D],
+    state float32 [n_seq, D] -> (y [n_seq, D] in the type of ``x``, the new state).  ``state_out`` may be
+    ``state`` itself; it is allocated when missing.  Without gradients: serving only."""
+    _check(x, "x")
+    _check(gate, "gate", like=x)
+    if x.dim() != 2:
+        raise ValueError("x must be [n_seq, D]")
+    if form not in _FORMS:
+        raise ValueError("form must be 'decay' or 'sigmoid'")
+    if not _no_grad(x, gate, state):
+        raise ValueError("gated_scan_step has no gradient: call it under torch.no_grad(), or gated_scan with one row a sequence")
+    _check_state(state, "state", x.shape)
+    if state is None or not state.is_contiguous():
+        raise ValueError("state must be contiguous")
+    y = _out(out, x.shape, x.dtype, x.device)
+    if state_out is None:
+        state_out = torch.empty_like(state)
+    elif _check_state(state_out, "state_out", x.shape) is not state and not state_out.is_contiguous():
+        raise ValueError("state_out must be contiguous")
+    n, d = x.shape
+    with _on(x.device, gate, state, state_out, y):
+        capi.check(capi.load().mfcc_gated_scan_step(n, d, _ROWS[x.dtype], _FORMS[form], x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0),
+                                                    state.data_ptr(), state_out.data_ptr(), y.data_ptr(), y.stride(0), _stream()))
+    return y, state_out
+
+
+# --------------------------------------------------------------------------
+# running normalisation
+# --------------------------------------------------------------------------
+def running_norm(feats, frame_counts=None, decay=0.995, state=None, eps=1e-5, center_only=False, out=None, dtype=None, state_out=None):
+    """Causal mean / variance normalisation of float32 rows, per sequence and column: row t is normalised by
+    the exponentially weighted mean and variance of the rows up to and including t,
+
+        w_t = decay w_{t-1} + 1,  m_t = m_{t-1} + (x_t - m_{t-1}) / w_t,  s_t = decay s_{t-1} + (x_t - m_{t-1}) (x_t - m_t)
+        y_t = (x_t - m_t) / sqrt(s_t / w_t + eps)          (``center_only``: y_t = x_t - m_t)
+
+    so it needs neither the whole utterance (``utterance_scalar_norm``) nor a corpus (``cmvn_apply``) and serves
+    live streams.  ``decay=1`` gives cumulative statistics (up to 2^24 rows).  ``state``: float32
+    [n_seq, 1 + 2 D] = (w, m, s) before the first row, default 0; :func:`running_norm_state` makes one from
+    corpus sums.  Returns (y, state behind the last row).  ``dtype``: type of y, float32 (default), bfloat16
+    or float16; ``out`` may be ``feats`` when that is float32; ``state_out`` is an array of its own.  Feature rows
+    have no gradient here: an input that requires one is refused."""
+    _check(feats, "feats", dtypes=(torch.float32,))
+    if not _no_grad(feats, state):
+        raise ValueError("running_norm has no gradient")
+    batch = _Batch(feats, frame_counts)
+    if not 0.0 < decay <= 1.0:
+        raise ValueError("decay must lie in (0, 1]")
+    dtype = (out.dtype if out is not None else torch.float32) if dtype is None else dtype
+    if dtype not in _ROWS:
+        raise ValueError("dtype must be float32, bfloat16 or float16")
+    shape = (batch.n_seq, 1 + 2 * batch.ncol)
+    state = _check_state(state, "state", shape)
+    y = _out(out, feats.shape, dtype, feats.device)
+    if state_out is None:
+        state_out = torch.empty(shape, dtype=torch.float32, device=feats.device)
+    elif not _check_state(state_out, "state_out", shape).is_contiguous():
+        raise ValueError("state_out must be contiguous")
+    if state is not None and state_out.data_ptr() == state.data_ptr() and state_out.numel():
+        raise ValueError("state_out must be an array of its own")
+    if state is not None and not state.is_contiguous():
+        state = state.contiguous()
+    with _on(feats.device, state, state_out, y):
+        ws = _workspace(batch, torch.float32, feats.device)
+        capi.check(capi.load().mfcc_running_norm(*batch.head(), decay, eps, int(bool(center_only)), _rows(feats), _ptr(state), _rows(y),
+                                                 _ROWS[dtype], state_out.data_ptr(), _ptr(ws), _stream()))
+    return y, state_out
+
+
+def running_norm_state(sums, weight, n_seq=1):
+    """State of :func:`running_norm` that starts from corpus statistics: ``sums`` = the float64 (n, sum x,
+    sum x^2) of ``cmvn_accumulate``, counted as ``weight`` rows -> float32 [n_seq, 1 + 2 D]."""
+    if sums.dim() != 1 or sums.numel() < 3 or sums.numel() % 2 == 0 or sums.dtype != torch.float64:
+        raise ValueError("sums must be a float64 vector of 1 + 2*D elements")
+    if not weight >= 0:
+        raise ValueError("weight must not be negative")
+    d = (sums.numel() - 1) // 2
+    mean = sums[1:1 + d] / sums[0]
+    var = (sums[1 + d:] / sums[0] - mean * mean).clamp(min=0)
+    row = torch.cat([torch.full_like(sums[:1], float(weight)), mean, weight * var]).to(torch.float32)
+    return row.repeat(n_seq, 1)
+
+
+# --------------------------------------------------------------------------
+# dropout
+# --------------------------------------------------------------------------
+def _drop(x, batch, per, threshold, seed, step, out):
+    y = _out(out, x.shape, x.dtype, x.device)
+    on_device = isinstance(step, torch.Tensor)
+    with _on(x.device, y, step if on_device else None):
+        capi.check(capi.load().mfcc_feature_dropout(*batch.head(), _ROWS[x.dtype], per, threshold, seed, 0 if on_device else step,
+                                                    step.data_ptr() if on_device else None, _rows(x), _rows(y), _stream()))
+    return y
+
+
+class _FeatureDropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, batch, per, threshold, seed, step):
+        on_device = isinstance(step, torch.Tensor)
+        ctx.save_for_backward(*((step,) if on_device else ()))   # a step changed in place before the backward pass is an error
+        ctx.call = batch, per, threshold, seed, None if on_device else step
+        return _drop(x, batch, per, threshold, seed, step, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        batch, per, threshold, seed, step = ctx.call
+        if gy.stride(-1) != 1 and gy.shape[-1] > 1:
+            gy = gy.contiguous()
+        return _drop(gy, batch, per, threshold, seed, ctx.saved_tensors[0] if step is None else step, None), None, None, None, None, None
+
+
+def feature_dropout(feats, p, seed, step=0, per="element", frame_counts=None, out=None):
+    """Zeroes a fraction ``p`` of the values and multiplies the others by 1 / (1 - p).  The mask is a function of
+    (seed, step, position) -- Philox4x32-10 blocks, 16 bits a decision, so ``p`` counts in steps of 2^-16 -- and is
+    never stored: the backward pass makes it again, and equal arguments give equal masks on every run.
+
+    ``per='element'``: every value on its own; ``'frame'``: whole rows; ``'sequence'``: a column for the
+    whole of a sequence, the mask a recurrent model keeps over time (``frame_counts`` tells the sequences of
+    packed rows).  Dropped values are 0 whatever they were, infinities and NaN included.  ``seed``: 0 ..
+    2^64 - 1; ``step``: an int 0 .. 2^63 - 1, or a one-element int64 device tensor that is read when the
+    kernel runs, for a captured graph whose replays draw new masks.  float32, bfloat16 or float16 rows
+    [rows, D] or [B, T, D]; all rows of a padded batch are processed.  ``out`` takes the result when no gradient is
+    asked for; it may be ``feats``."""
+    _check(feats, "feats")
+    if per not in _PER:
+        raise ValueError("per must be 'element', 'frame' or 'sequence'")
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("p must lie in [0, 1]")
+    if not 0 <= seed < 1 << 64:
+        raise ValueError("seed must lie in 0 .. 2^64 - 1")
+    if isinstance(step, torch.Tensor):
+        if not step.is_cuda or step.dtype != torch.int64 or step.numel() != 1:
+            raise ValueError("step must be an int or a one-element int64 device tensor")
+    elif not 0 <= step < 1 << 63:
+        raise ValueError("step must lie in 0 .. 2^63 - 1")
+    batch = _Batch(feats, frame_counts)
+    args = batch, _PER[per], int(round(p * 65536)), seed, step
+    if _no_grad(feats):
+        return _drop(feats, *args, out)
+    if out is not None:
+        raise ValueError("out is for calls without gradients")
+    return _FeatureDropout.apply(feats, *args)

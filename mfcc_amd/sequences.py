@@ -13,6 +13,7 @@ import torch
 
 from . import _capi as capi
 from .frontend import MFCC, _on, _ptr, _stream_ptr, frames_layout
+from .recurrent import feature_dropout
 
 
 def _frames_layout(feats, frame_counts):
@@ -59,11 +60,16 @@ def pad_sequences(feats, frame_counts, maxlen=None, padding="post", truncating="
     return out, frame_counts.copy()
 
 
-def ctc_feature_batch(audios, variant="self5", time_steps=None, normalize=True, device=None, **overrides):
+def ctc_feature_batch(audios, variant="self5", time_steps=None, normalize=True, device=None, dropout=0.0, seed=None, step=0, **overrides):
     """Feature side of create_minibatch_ctc (inference_ctc_eri_05.py:283-300): a list of
     utterances (int16 / float arrays of any lengths) -> (features [B, T, 39], seq_length
     int64[B]) with per-utterance scalar normalisation and zero padding: three launches on a
-    repeated batch shape (the offset tables of a new shape are uploaded once and cached)."""
+    repeated batch shape (the offset tables of a new shape are uploaded once and cached).
+    ``dropout``: the share of the coefficients that each utterance loses for its whole length, the
+    others scaled up (``feature_dropout`` with ``per='sequence'``, in place before the padding);
+    the mask is a function of ``seed``, which it needs, and of ``step``, e.g. the training step."""
+    if dropout and seed is None:
+        raise ValueError("dropout needs a seed")
     fe = MFCC(variant, device=device, **overrides)
     lengths = [int(np.asarray(a).shape[-1]) if not isinstance(a, torch.Tensor) else int(a.shape[-1]) for a in audios]
     parts = [a if isinstance(a, torch.Tensor) else torch.as_tensor(np.ascontiguousarray(a)) for a in audios]
@@ -74,4 +80,6 @@ def ctc_feature_batch(audios, variant="self5", time_steps=None, normalize=True, 
     counts = np.diff(lay.frame_offsets)
     if normalize:
         utterance_scalar_norm(feats, counts)
+    if dropout:
+        feature_dropout(feats, dropout, seed, step=step, per="sequence", frame_counts=counts, out=feats)
     return pad_sequences(feats, counts, maxlen=time_steps)
