@@ -1,5 +1,6 @@
 // C entry points of the operators along time (see "operators along time over feature rows" in include/mfcc_amd.h).
 #include <algorithm>
+#include <type_traits>
 
 #include "abi.h"
 #include "sequence_kernels.h"
@@ -11,6 +12,7 @@ using mfcc::Rows;
 namespace {
 
 constexpr int64_t kMaxColumns = 1 << 20;
+constexpr int64_t kMaxRows = 1 << 30;  // of one sequence: row numbers inside it are 32-bit
 
 // The geometry of a call, checked once: 0 or a negative error code.
 struct Shape {
@@ -25,8 +27,7 @@ int shape_of(const char* who, const mfcc_layout* layout, int64_t n_seq, int64_t 
   out->b = Batch{layout ? layout->d_frame_off : nullptr, n_seq, time_steps, ncol, reverse};
   out->longest = layout ? (time_steps ? std::min(layout->longest, time_steps) : layout->longest) : time_steps;
   out->rows = time_steps || !layout ? n_seq * time_steps : layout->total_frames;
-  if (out->longest > INT32_MAX) return fail(MFCC_ERR_UNSUPPORTED, "%s: a sequence of more than 2^31-1 rows", who);
-  if (!layout && time_steps == 0) out->b.n_seq = n_seq;  // sequences without rows: states pass through
+  if (out->longest > kMaxRows) return fail(MFCC_ERR_UNSUPPORTED, "%s: a sequence of more than 2^30 rows", who);
   return MFCC_OK;
 }
 
@@ -46,9 +47,54 @@ int check_rows(const char* who, const char* name, const mfcc_rows* r, const Shap
   return MFCC_OK;
 }
 
+// How workgroups divide sequences, columns and time.  It depends on the shape of the batch alone, so that the backward
+// pass finds its checkpoints whatever the alignment of its arrays.
+struct Grid {
+  int v, tile_rows;
+  mfcc::Split w;
+  dim3 blocks;
+};
+Grid grid_of(const Shape& s) {
+  Grid g;
+  g.v = s.b.ncol % 2 ? 1 : 2;   // values of a row that a thread takes at once
+  const int rows = mfcc::kSlotRows;
+  g.w.groups = s.b.ncol / g.v;
+  // column blocks of at most a wave's width, equally wide
+  const int nb = (g.w.groups + 63) / 64;
+  g.w.cb = (g.w.groups + nb - 1) / nb;
+  // slots of time: as many as the threads give, at most 64 (each thread composes the maps of all of them), and no more
+  // than the longest sequence fills; what is left over takes further sequences
+  const int slots = mfcc::kSeqThreads / g.w.cb;
+  const int64_t need = std::max<int64_t>(1, (s.longest + rows - 1) / rows);
+  g.w.per = (int32_t)std::min<int64_t>(std::min(slots, 64), need);
+  g.w.seqs = need <= g.w.per ? slots / g.w.per : 1;
+  g.tile_rows = g.w.per * rows;
+  g.blocks = dim3(blocks_for(s.b.n_seq, g.w.seqs), (unsigned)nb);
+  return g;
+}
+
+bool aligned(const mfcc_rows* r, const Shape& s, int v, size_t size) {
+  return !r || (((uintptr_t)r->data % (v * size)) == 0 && r->row_stride % v == 0 && (s.b.steps == 0 || r->seq_stride % v == 0));
+}
+
+// f(type's zero, number of values, aligned) for the row type, the values a thread takes and the alignment of the arrays
+template <typename T, typename F>
+void dispatch_pack(int v, bool al, F f) {
+  if (v == 1) f((T)0.0f, std::integral_constant<int, 1>(), std::true_type());
+  else if (al) f((T)0.0f, std::integral_constant<int, 2>(), std::true_type());
+  else f((T)0.0f, std::integral_constant<int, 2>(), std::false_type());
+}
+template <typename F>
+void dispatch(int32_t dtype, int v, bool al, F f) {
+  if (dtype == MFCC_ROWS_F32) dispatch_pack<float>(v, al, f);
+  else if (dtype == MFCC_ROWS_BF16) dispatch_pack<mfcc::bf16>(v, al, f);
+  else dispatch_pack<mfcc::f16>(v, al, f);
+}
+
+// The array of rows for a kernel; null where the batch has no rows.
 template <typename T>
-Rows<T> rows_of(const mfcc_rows* r) {
-  return r ? Rows<T>{(T*)r->data, r->seq_stride, r->row_stride} : Rows<T>{nullptr, 0, 0};
+Rows<T> rows_of(const mfcc_rows* r, const Shape& s) {
+  return r && s.rows > 0 ? Rows<T>{(T*)r->data, r->seq_stride, r->row_stride} : Rows<T>{nullptr, 0, 0};
 }
 
 int bad_dtype(const char* who, int32_t dtype) { return fail(MFCC_ERR_INVALID, "%s: rows type %d", who, dtype); }
@@ -61,7 +107,7 @@ int64_t mfcc_gated_scan_checkpoints(const mfcc_layout* layout, int64_t n_seq, in
   Shape s;
   if (const int rc = shape_of("mfcc_gated_scan_checkpoints", layout, n_seq, time_steps, ncol, 0, &s)) return rc;
   if (rows_dtype < 0 || rows_dtype > MFCC_ROWS_F16) return bad_dtype("mfcc_gated_scan_checkpoints", rows_dtype);
-  const int64_t k = mfcc::kScanTile;
+  const int64_t k = grid_of(s).tile_rows;
   return (time_steps || !layout ? s.b.n_seq * ((time_steps + k - 1) / k) : s.rows / k + s.b.n_seq) * ncol;
 }
 
@@ -82,21 +128,18 @@ int mfcc_gated_scan(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps
   if (const int rc = check_rows(who, "x", x, s, false)) return rc;
   if (const int rc = check_rows(who, "gate", gate, s, false)) return rc;
   if (const int rc = check_rows(who, "y", y, s, true)) return rc;
-  const int64_t total = s.b.n_seq * ncol;
-  if (total == 0) return MFCC_OK;
+  if (rows_dtype < 0 || rows_dtype > MFCC_ROWS_F16) return bad_dtype(who, rows_dtype);
+  if (s.b.n_seq == 0) return MFCC_OK;
   const mfcc::ScanPtrs q{h0, nullptr, last, checkpoints, nullptr};
-  auto go = [&](auto zero) {
+  const Grid c = grid_of(s);
+  const size_t size = rows_dtype == MFCC_ROWS_F32 ? 4 : 2;
+  const bool al = aligned(x, s, c.v, size) && aligned(gate, s, c.v, size) && aligned(y, s, c.v, size);
+  dispatch(rows_dtype, c.v, al, [&](auto zero, auto v, auto al) {
     using T = decltype(zero);
-    auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_kernel<T, true> : mfcc::gated_scan_kernel<T, false>;
-    hipLaunchKernelGGL(k, dim3(blocks_for(total, 256)), dim3(256), 0, (hipStream_t)stream, s.b, rows_of<const T>(x), rows_of<const T>(gate),
-                       rows_of<T>(y), q);
-  };
-  switch (rows_dtype) {
-    case MFCC_ROWS_F32: go(0.0f); break;
-    case MFCC_ROWS_BF16: go((mfcc::bf16)0.0f); break;
-    case MFCC_ROWS_F16: go((mfcc::f16)0.0f); break;
-    default: return bad_dtype(who, rows_dtype);
-  }
+    auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_kernel<T, v(), al(), true> : mfcc::gated_scan_kernel<T, v(), al(), false>;
+    hipLaunchKernelGGL(k, c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const T>(x, s), rows_of<const T>(gate, s),
+                       rows_of<T>(y, s), q);
+  });
   HIP_TRY(hipGetLastError());
   return MFCC_OK;
 }
@@ -116,21 +159,19 @@ int mfcc_gated_scan_backward(const mfcc_layout* layout, int64_t n_seq, int64_t t
   if (const int rc = check_rows(who, "grad_x", grad_x, s, true)) return rc;
   if (const int rc = check_rows(who, "grad_gate", grad_gate, s, true)) return rc;
   if (!checkpoints && s.rows > 0) return fail(MFCC_ERR_INVALID, "%s: checkpoints is null", who);
-  const int64_t total = s.b.n_seq * ncol;
-  if (total == 0) return MFCC_OK;
+  if (rows_dtype < 0 || rows_dtype > MFCC_ROWS_F16) return bad_dtype(who, rows_dtype);
+  if (s.b.n_seq == 0) return MFCC_OK;
   const mfcc::ScanPtrs q{nullptr, grad_last, nullptr, const_cast<float*>(checkpoints), grad_h0};
-  auto go = [&](auto zero) {
+  const Grid c = grid_of(s);
+  const size_t size = rows_dtype == MFCC_ROWS_F32 ? 4 : 2;
+  const bool al = aligned(x, s, c.v, size) && aligned(gate, s, c.v, size) && aligned(grad_y, s, c.v, size) && aligned(grad_x, s, c.v, size) &&
+            aligned(grad_gate, s, c.v, size);
+  dispatch(rows_dtype, c.v, al, [&](auto zero, auto v, auto al) {
     using T = decltype(zero);
-    auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_backward_kernel<T, true> : mfcc::gated_scan_backward_kernel<T, false>;
-    hipLaunchKernelGGL(k, dim3(blocks_for(total, 256)), dim3(256), 0, (hipStream_t)stream, s.b, rows_of<const T>(x), rows_of<const T>(gate),
-                       rows_of<const T>(grad_y), rows_of<T>(grad_x), rows_of<T>(grad_gate), q);
-  };
-  switch (rows_dtype) {
-    case MFCC_ROWS_F32: go(0.0f); break;
-    case MFCC_ROWS_BF16: go((mfcc::bf16)0.0f); break;
-    case MFCC_ROWS_F16: go((mfcc::f16)0.0f); break;
-    default: return bad_dtype(who, rows_dtype);
-  }
+    auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_backward_kernel<T, v(), al(), true> : mfcc::gated_scan_backward_kernel<T, v(), al(), false>;
+    hipLaunchKernelGGL(k, c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const T>(x, s), rows_of<const T>(gate, s),
+                       rows_of<const T>(grad_y, s), rows_of<T>(grad_x, s), rows_of<T>(grad_gate, s), q);
+  });
   HIP_TRY(hipGetLastError());
   return MFCC_OK;
 }
@@ -175,7 +216,7 @@ int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_ste
   auto go = [&](auto zero) {
     using T = decltype(zero);
     hipLaunchKernelGGL(mfcc::running_norm_kernel<T>, dim3(blocks_for(total, 256)), dim3(256), 0, (hipStream_t)stream, s.b,
-                       rows_of<const float>(x), rows_of<T>(y), decay, (float)eps, center_only ? 1 : 0, state_in, state_out);
+                       rows_of<const float>(x, s), rows_of<T>(y, s), decay, (float)eps, center_only ? 1 : 0, state_in, state_out);
   };
   switch (y_dtype) {
     case MFCC_ROWS_F32: go(0.0f); break;
@@ -204,7 +245,7 @@ int mfcc_feature_dropout(const mfcc_layout* layout, int64_t n_seq, int64_t time_
   auto go = [&](auto zero) {
     using T = decltype(zero);
     hipLaunchKernelGGL(mfcc::feature_dropout_kernel<T>, dim3(blocks_for(total, 256)), dim3(256), 0, (hipStream_t)stream, s.b, s.rows, per,
-                       (uint32_t)threshold, scale, seed, step, step_device, rows_of<const T>(x), rows_of<T>(y));
+                       (uint32_t)threshold, scale, seed, step, step_device, rows_of<const T>(x, s), rows_of<T>(y, s));
   };
   switch (rows_dtype) {
     case MFCC_ROWS_F32: go(0.0f); break;
