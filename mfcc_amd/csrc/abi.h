@@ -30,6 +30,7 @@ struct mfcc_layout {
   std::vector<int64_t> sample_off, frame_off;
   int64_t* d_sample_off = nullptr;
   int64_t* d_frame_off = nullptr;
+  int64_t* d_order = nullptr;  // utterances by falling frame count, behind the offsets in the same allocation; frames_only layouts of unequal counts
   mfcc::Tile* d_tiles = nullptr;
   int64_t n_tiles;
   // the same frames cut for the persistent workgroups of split_kernel.h: workgroup w walks

@@ -1013,7 +1013,18 @@ int mfcc_layout_create_frames(int device, const int64_t* frame_counts_host, int6
     l->frames_only = true;
     hipError_t e = hipSetDevice(device);
     int rc = e == hipSuccess ? MFCC_OK : fail(MFCC_ERR_HIP, "hipSetDevice: %s", hipGetErrorString(e));
-    if (!rc) rc = upload(l->frame_off, &l->d_frame_off);
+    if (!rc) {
+      std::vector<int64_t> table(l->frame_off);
+      const bool ragged = std::any_of(frame_counts_host, frame_counts_host + n_utts, [&](int64_t n) { return n != l->longest; });
+      if (ragged) {
+        table.resize(2 * n_utts + 1);
+        std::iota(table.begin() + n_utts + 1, table.end(), (int64_t)0);
+        std::stable_sort(table.begin() + n_utts + 1, table.end(),
+                         [&](int64_t a, int64_t b) { return frame_counts_host[a] > frame_counts_host[b]; });
+      }
+      rc = upload(table, &l->d_frame_off);
+      if (!rc && ragged) l->d_order = l->d_frame_off + n_utts + 1;
+    }
     if (rc) {
       mfcc_layout_destroy(l);
       return rc;

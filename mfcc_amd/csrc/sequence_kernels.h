@@ -21,6 +21,7 @@ struct Rows {
 
 struct Batch {
   const int64_t* off;  // packed rows / lengths; nullptr: steps rows each
+  const int64_t* order;  // the sequences by falling length, so that the longest start first; nullptr: as they come
   int64_t n_seq;
   int64_t steps;       // 0 = packed
   int32_t ncol;
@@ -50,9 +51,16 @@ __device__ inline T* row_base(const Rows<T>& r, const Batch& b, int64_t u, const
 constexpr int kSeqThreads = 512;
 constexpr int kSlotRows = 8;   // R: composing costs per / R steps a value, registers 2 .. 6 R V
 
+// Where the sequences and columns are too few for the card, a sequence is also cut into `pieces` of `piece_tiles` tiles, a
+// workgroup each: a first kernel composes every piece into one entry of a workspace, the second one composes the entries before its
+// piece and goes on from there (the rows are read twice, mostly from the caches the second time).
 struct Split {
   int32_t groups, cb;    // column groups of a row, of a workgroup
+  int32_t column_blocks; // workgroups to a row
+  int32_t blocks;        // workgroups to a column block
   int32_t seqs, per;     // sequences of a workgroup, time slots of a sequence
+  int32_t pieces, piece_tiles;  // pieces > 1 only with seqs == 1
+  int32_t near;          // the rows of a tile lie within 4 GiB in every array
 };
 
 // V neighbouring values of a row; AL: rows are aligned to all of them, one access.
@@ -82,78 +90,130 @@ __device__ inline void store_pack(T* p, const float* f) {
   }
 }
 
+// A value that all lanes agree on, in scalar registers.
+__device__ inline int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ inline int64_t scalar(int64_t v) {
+  return (int64_t)((uint64_t)(uint32_t)scalar((int)v) | (uint64_t)(uint32_t)scalar((int)(v >> 32)) << 32);
+}
+
 // What a thread works on.  Threads behind the last slot or column group are doubles of others: they compute and write the
 // same values, so that no access to rows needs a predicate as long as a tile is full.
 struct Seat {
   int64_t u;           // sequence
   Span s;
   int n, sub, slot, cg, col;
+  int piece, tile, tiles, full;  // the tiles [tile, tiles) of the sequence, those below `full` without a missing row
   bool on;             // there is such a sequence
+  bool there;          // the workgroup has something to do
 };
 template <int V>
-__device__ inline Seat seat_of(const Batch& b, const Split& w, int64_t block, int column_block) {
+__device__ inline Seat seat_of(const Batch& b, const Split& w) {
   Seat t;
+  // Workgroups go to the 8 XCDs in turn: the column blocks of the same rows are 8 apart, so that they run on one
+  // XCD at about the same time and share the cache lines at their borders (2048 x 512 rows of 257 floats: 2270 -> 4500 GB/s).
+  const int eight = blockIdx.x / (8 * w.column_blocks), r = blockIdx.x - eight * 8 * w.column_blocks;
+  const int column_block = r / 8, at = eight * 8 + r % 8, block = at / w.pieces;
+  t.there = at < w.blocks;
+  t.piece = at - block * w.pieces;
   t.slot = threadIdx.x / w.cb;
   t.cg = min((int)threadIdx.x - t.slot * w.cb, w.groups - 1 - column_block * w.cb);
   if (t.slot >= w.seqs * w.per) t.slot = 0;
-  const int g = t.slot / w.per;
-  t.sub = t.slot - g * w.per;
-  t.u = block * w.seqs + g;
   t.col = (column_block * w.cb + t.cg) * V;
-  t.on = t.u < b.n_seq;
-  t.s = t.on ? span_of(b, t.u) : Span{0, 0};
-  t.n = (int)t.s.n;    // the same for all threads where a workgroup has one sequence: its tile loop runs in step
+  const int tile_rows = w.per * kSlotRows;
+  if (w.seqs > 1) {     // several sequences of one tile
+    const int g = t.slot / w.per;
+    t.sub = t.slot - g * w.per;
+    t.u = (int64_t)block * w.seqs + g;
+    t.on = t.u < b.n_seq;
+    t.s = t.on ? span_of(b, t.u) : Span{0, 0};
+    t.n = (int)t.s.n;
+    t.tile = 0, t.tiles = 1, t.full = 0;
+  } else {              // one sequence: everything but sub and the columns is the same for all threads, in scalar registers
+    t.sub = t.slot;
+    t.on = t.there;
+    t.u = t.there ? b.order ? b.order[block] : block : 0;
+    t.s = span_of(b, t.u);
+    t.n = (int)t.s.n;
+    t.tile = t.piece * w.piece_tiles;
+    t.tiles = min((t.n + tile_rows - 1) / tile_rows, t.tile + w.piece_tiles);
+    t.full = w.near ? max(min(t.n / tile_rows, t.tiles), t.tile) : t.tile;
+  }
+  t.tile = scalar(t.tile), t.tiles = scalar(t.tiles), t.full = scalar(t.full);
   return t;
 }
 
-// Where a thread reads the rows of its sequence from; one without rows reads the first row of the array instead (a batch
-// without any rows has null arrays, and nothing is read).
+// Rows of one sequence in any order of visit.  Full tiles: the address is a base that all threads share (scalar registers)
+// plus 32 bits of the thread that never change, so a row costs no vector arithmetic.  Otherwise rows behind the end
+// repeat the last one, and a thread without rows reads the first row of the array (a batch without any rows has null
+// arrays, and nothing is read).  No branch in either form, so that the loads of the next tile go out while the
+// current one is worked on; loads behind a store would have to wait for it (vmcnt counts both in order).
 template <typename T>
-struct Source {
-  const T* p;
-  int64_t rs;
-  int last;
+struct Lane {
+  const T* p;            // row 0 of the visit, the thread's column
+  int64_t rs;            // to the next row of the visit
+  const char* base;      // lowest row of tile 0, column 0
+  int64_t tile_step, row_step;   // bytes
+  uint32_t off;
 };
-template <typename T>
-__device__ inline Source<T> source_of(const Rows<const T>& r, const Batch& b, const Seat& t) {
-  if (t.n == 0) return Source<T>{r.p, 0, 0};
-  return Source<T>{row_base(r, b, t.u, t.s) + t.col, b.reverse ? -r.rs : r.rs, t.n - 1};
+template <int V, typename T>
+__device__ inline Lane<T> lane_of(const Rows<T>& r, const Batch& b, const Split& w, const Seat& t) {
+  Lane<T> f;
+  const int64_t first = (b.steps ? t.u * r.ss : 0) + (t.s.first + (b.reverse ? t.n - 1 : 0)) * r.rs;
+  f.rs = t.n == 0 ? 0 : b.reverse ? -r.rs : r.rs;
+  f.p = r.p + (t.n == 0 ? 0 : first + t.col);
+  // slots of a tile upwards in memory: the last one comes first in reverse (used where a workgroup has one sequence)
+  f.base = (const char*)(r.p + scalar(first - (b.reverse ? (int64_t)(w.per - 1) * kSlotRows * r.rs : 0)));
+  f.row_step = (b.reverse ? -r.rs : r.rs) * (int64_t)sizeof(T);
+  f.tile_step = f.row_step * (w.per * kSlotRows);
+  f.off = ((b.reverse ? w.per - 1 - t.sub : t.sub) * kSlotRows * (uint32_t)r.rs + t.col) * (uint32_t)sizeof(T);
+  return f;
 }
-// R rows from row t0 on.  FULL: they all exist; otherwise rows behind the end repeat the last one.  Without a branch, so
-// that the loads of the next tile go out while the current one is worked on.
-template <bool FULL, bool AL, typename T, int V, int R>
-__device__ inline void load_rows(Pack<T, V> (&r)[R], const Source<T>& f, int t0) {
-  const T* p = f.p + (FULL ? t0 : min(t0, f.last)) * f.rs;
+template <bool FULL, bool AL, typename T, typename S, int V>
+__device__ inline void load_rows(Pack<T, V> (&r)[kSlotRows], const Lane<S>& f, const Seat& t, const Split& w, int tile) {
+  if constexpr (FULL) {
+    const char* p = f.base + tile * f.tile_step;
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    load_pack<AL>(r[i], p);
-    p += FULL || t0 + i < f.last ? f.rs : 0;
+    for (int i = 0; i < kSlotRows; ++i, p += f.row_step) load_pack<AL>(r[i], (const T*)(p + f.off));
+  } else {
+    const int t0 = (tile * w.per + t.sub) * kSlotRows, last = max(t.n - 1, 0);
+    const T* p = f.p + min(t0, last) * f.rs;
+#pragma unroll
+    for (int i = 0; i < kSlotRows; ++i) {
+      load_pack<AL>(r[i], p);
+      p += t0 + i < last ? f.rs : 0;
+    }
   }
+}
+// Where row r of the thread's slot goes.
+template <bool FULL, typename T>
+__device__ inline T* row_at(const Lane<T>& f, const Seat& t, const Split& w, int tile, int r) {
+  if constexpr (FULL) return (T*)(f.base + tile * f.tile_step + r * f.row_step + f.off);
+  return (T*)f.p + ((tile * w.per + t.sub) * kSlotRows + r) * f.rs;
 }
 
 template <bool AL, int V, typename T>
-__device__ inline void zero_behind(const Rows<T>& y, const Batch& b, const Seat& t, int per) {
+__device__ inline void zero_behind(const Rows<T>& y, const Batch& b, const Split& w, const Seat& t) {
   const float z[V] = {};
-  for (int64_t r = t.n + t.sub; r < b.steps; r += per) store_pack<AL, V>(y.p + t.u * y.ss + r * y.rs + t.col, z);
+  for (int64_t r = t.n + t.piece * w.per + t.sub; r < b.steps; r += w.pieces * w.per) store_pack<AL, V>(y.p + t.u * y.ss + r * y.rs + t.col, z);
 }
 
 // ---- gated recurrence -----------------------------------------------------------------------------
 // h_t = a_t h_{t-1} + b_t is a composition of maps h -> A h + X: a run of rows is one such map, and maps of neighbouring
 // runs join to (A2 A1, A2 X1 + X2).  Bound: HBM, 3 values moved a value forward and 5 backward.
 
-// a = 1 / (1 + exp(-g)) and 1 - a without cancellation, from e = exp(-|g|).  The hardware exponential and reciprocal
-// are good to one unit in the last place, and the product with log2(e) adds |g| 2^-24.
+// a = 1 / (1 + e) and 1 - a = e a from e = exp(-g), neither by a difference.  g is held above -87 so that e stays finite (a is
+// 2^-125 there; a NaN stays one).  The hardware exponential and reciprocal are good to one unit in the last place, and the
+// product with log2(e) adds |g| 2^-24.
 __device__ inline void sigmoid2(float g, float& a, float& na) {
-  const float e = __expf(-fabsf(g));
-  const float r = __builtin_amdgcn_rcpf(1.0f + e);
-  const float er = e * r;
-  a = g >= 0.0f ? r : er;
-  na = g >= 0.0f ? er : r;
+  const float e = __expf(-(g < -87.0f ? -87.0f : g));
+  a = __builtin_amdgcn_rcpf(1.0f + e);
+  na = e * a;
 }
 
 struct ScanPtrs {
   const float *h0, *glast;
   float *last, *ckpt, *gh0;
+  float2* maps;   // [sequence][piece][column] where sequences are cut into pieces
 };
 
 // Checkpoint of (sequence, tile): float32 states that enter a tile.  Packed sequences get rows / K + u as their first one:
@@ -166,10 +226,95 @@ template <typename T, int V>
 struct ScanRows {
   Pack<T, V> x[kSlotRows], g[kSlotRows];
 };
-template <bool FULL, bool AL, typename T, int V>
-__device__ inline void load_tile(ScanRows<T, V>& r, const Source<T>& fx, const Source<T>& fg, int t0) {
-  load_rows<FULL, AL>(r.x, fx, t0);
-  load_rows<FULL, AL>(r.g, fg, t0);
+
+// The map of every piece: forward h -> A h + X from (x, gate), backward e -> A e + E from (gate, grad_y). A slot takes a contiguous
+// run of the piece, so that the threads meet once.
+template <typename T, int V, bool AL, bool SIG, bool BACK>
+__global__ void __launch_bounds__(kSeqThreads, 4) gated_scan_pieces_kernel(const Batch b, const Split w, const Rows<const T> x,
+                                                                           const Rows<const T> g, const ScanPtrs q) {
+  constexpr int R = kSlotRows;
+  __shared__ float2 maps[kSeqThreads * V];
+  const Seat t = seat_of<V>(b, w);
+  if (!t.there || t.tile >= t.tiles || !g.p) return;   // the same for the whole workgroup
+  const bool no_gy = BACK && !x.p;
+  const Lane<const T> fg = lane_of<V>(g, b, w, t), fx = no_gy ? fg : lane_of<V>(x, b, w, t);
+  float A[V], X[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) A[v] = 1.0f, X[v] = 0.0f;
+  const int run = w.piece_tiles * R, first = t.tile * w.per * R + t.sub * run;
+  const int len = min(max(t.n - first, 0), run), last = BACK ? (len + R - 1) / R * R - R : 0;
+  auto load = [&](ScanRows<T, V>& r, int at) {
+    const T *px = fx.p + min(first + at, t.n - 1) * fx.rs, *pg = fg.p + min(first + at, t.n - 1) * fg.rs;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      load_pack<AL>(r.x[i], px);
+      load_pack<AL>(r.g[i], pg);
+      px += first + at + i < t.n - 1 ? fx.rs : 0;
+      pg += first + at + i < t.n - 1 ? fg.rs : 0;
+    }
+  };
+  ScanRows<T, V> in, next;
+  load(in, last);
+  for (int i = 0; i < len; i += R) {
+    const int at = BACK ? last - i : i, k = len - at;
+    load(next, BACK ? max(at - R, 0) : at + R);
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int r = BACK ? R - 1 - j : j;
+        float a = (float)in.g[r].v[v], na = 1.0f;
+        if constexpr (SIG) sigmoid2(a, a, na);
+        const float xv = no_gy ? 0.0f : (float)in.x[r].v[v];
+        const float nx = BACK ? a * (xv + X[v]) : fmaf(a, X[v], na * xv);
+        X[v] = r < k ? nx : X[v];
+        A[v] = r < k ? A[v] * a : A[v];
+      }
+    in = next;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) maps[(t.slot * V + v) * w.cb + t.cg] = make_float2(A[v], X[v]);
+  __syncthreads();
+  if (t.sub == 0) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float2 f = make_float2(1.0f, 0.0f);
+      for (int s = 0; s < w.per; ++s) {
+        const float2 e = maps[((BACK ? w.per - 1 - s : s) * V + v) * w.cb + t.cg];
+        f = make_float2(e.x * f.x, fmaf(e.x, f.y, e.y));
+      }
+      q.maps[(t.u * w.pieces + t.piece) * b.ncol + t.col + v] = f;
+    }
+  }
+}
+
+// What enters a piece: the maps of the `count` pieces on the way to it, in order, on the state `h`.  Each slot composes a run of them,
+// the slots meet in LDS.  `base` is the first map, `step` the distance to the next.
+template <int V>
+__device__ inline void enter_piece(float (&h)[V], const float2* base, int64_t step, int count, const Split& w, const Seat& t, float2* maps) {
+  if (count == 0) return;
+  const int run = (count + w.per - 1) / w.per, lo = t.sub * run, hi = min(lo + run, count);
+  float2 f[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) f[v] = make_float2(1.0f, 0.0f);
+  const float2* p = base + lo * step;
+#pragma unroll 8
+  for (int i = lo; i < hi; ++i, p += step)
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float2 e = p[v];
+      f[v] = make_float2(e.x * f[v].x, fmaf(e.x, f[v].y, e.y));
+    }
+#pragma unroll
+  for (int v = 0; v < V; ++v) maps[(t.slot * V + v) * w.cb + t.cg] = f[v];
+  __syncthreads();
+  for (int s = 0; s < w.per; ++s)
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float2 e = maps[(s * V + v) * w.cb + t.cg];
+      h[v] = fmaf(e.x, h[v], e.y);
+    }
+  __syncthreads();
 }
 
 template <typename T, int V, bool AL, bool SIG>
@@ -177,28 +322,21 @@ __global__ void __launch_bounds__(kSeqThreads, 4) gated_scan_kernel(const Batch 
                                                                     const Rows<T> y, const ScanPtrs q) {
   constexpr int R = kSlotRows;
   __shared__ float2 maps[2][kSeqThreads * V];
-  const Seat t = seat_of<V>(b, w, blockIdx.x, blockIdx.y);
-  const Source<T> fx = source_of(x, b, t), fg = source_of(g, b, t);
-  const int64_t ys = b.reverse ? -y.rs : y.rs;
-  T* const yp = row_base(y, b, t.u, t.s) + t.col;
-  const int tile_rows = w.per * R;
+  const Seat t = seat_of<V>(b, w);
+  if (!t.there) return;
+  const Lane<const T> fx = lane_of<V>(x, b, w, t), fg = lane_of<V>(g, b, w, t);
+  const Lane<T> fy = lane_of<V>(y, b, w, t);
   const int64_t end = t.u * b.ncol + t.col;   // of the states of a sequence
-  float carry[V] = {};
+  float carry[V] = {}, h[V] = {};
   if (t.on && q.h0)
 #pragma unroll
     for (int v = 0; v < V; ++v) carry[v] = q.h0[end + v];
-  if (t.on && t.n == 0 && q.last)
-#pragma unroll
-    for (int v = 0; v < V; ++v) q.last[end + v] = carry[v];
-  float* const ck = q.ckpt ? q.ckpt + checkpoint_row(b, t, tile_rows) * b.ncol + t.col : nullptr;
+  float* const ck = q.ckpt ? q.ckpt + checkpoint_row(b, t, w.per * R) * b.ncol + t.col : nullptr;
 
   auto work = [&](auto full, const ScanRows<T, V>& in, int tile) {
     constexpr bool FULL = full();
-    const int t0 = (tile * w.per + t.sub) * R;
-    const int k = FULL ? R : min(max(t.n - t0, 0), R);
+    const int k = FULL ? R : min(max(t.n - (tile * w.per + t.sub) * R, 0), R);
     float a[R][V], x1[R][V], A[V], X[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) A[v] = 1.0f, X[v] = 0.0f;
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -214,7 +352,6 @@ __global__ void __launch_bounds__(kSeqThreads, 4) gated_scan_kernel(const Batch 
         X[v] = r ? fmaf(a[r][v], X[v], x1[r][v]) : x1[r][v];
         A[v] = r ? A[v] * a[r][v] : a[r][v];
       }
-    float h[V];
     if (w.per > 1) {
       float2* const m = maps[tile & 1];
 #pragma unroll
@@ -234,40 +371,47 @@ __global__ void __launch_bounds__(kSeqThreads, 4) gated_scan_kernel(const Batch 
 #pragma unroll
       for (int v = 0; v < V; ++v) h[v] = carry[v], carry[v] = fmaf(A[v], carry[v], X[v]);
     }
-    if (FULL || k > 0) {
-      if (ck && t.sub == 0)
+    if (ck && t.sub == 0 && k > 0)
 #pragma unroll
-        for (int v = 0; v < V; ++v) ck[(int64_t)tile * b.ncol + v] = h[v];
-      T* o = yp + t0 * ys;
+      for (int v = 0; v < V; ++v) ck[(int64_t)tile * b.ncol + v] = h[v];
 #pragma unroll
-      for (int r = 0; r < R; ++r, o += ys) {
+    for (int r = 0; r < R; ++r) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = fmaf(a[r][v], h[v], x1[r][v]);
-        if (FULL || r < k) store_pack<AL, V>(o, h);
-      }
-      if (t0 + k == t.n && q.last)
-#pragma unroll
-        for (int v = 0; v < V; ++v) q.last[end + v] = h[v];
+      for (int v = 0; v < V; ++v) h[v] = fmaf(a[r][v], h[v], x1[r][v]);
+      if (FULL || r < k) store_pack<AL, V>(row_at<FULL>(fy, t, w, tile, r), h);
     }
   };
 
-  if (!x.p) return;
-  ScanRows<T, V> in, next;
-  const int full = w.seqs > 1 ? 0 : t.n / tile_rows, first = t.sub * R;
-  load_tile<false, AL>(in, fx, fg, first);
-  int tile = 0;
-  for (; tile + 1 < full; ++tile) {
-    load_tile<true, AL>(next, fx, fg, first + (tile + 1) * tile_rows);
-    work(std::true_type(), in, tile);
-    in = next;
+  if (x.p && t.tile < t.tiles) {   // the same for the whole workgroup
+    ScanRows<T, V> in, next;
+    auto load = [&](auto full, ScanRows<T, V>& r, int tile) {
+      load_rows<full(), AL>(r.x, fx, t, w, tile);
+      load_rows<full(), AL>(r.g, fg, t, w, tile);
+    };
+    int tile = t.tile;
+    load(std::false_type(), in, tile);
+    if (t.piece > 0) enter_piece(carry, q.maps + t.u * w.pieces * b.ncol + t.col, b.ncol, t.piece, w, t, maps[0]);
+    for (; tile + 1 < t.full; ++tile) {
+      load(std::true_type(), next, tile + 1);
+      work(std::true_type(), in, tile);
+      in = next;
+    }
+    if (tile < t.full) {
+      if (t.full < t.tiles) load(std::false_type(), next, t.full);
+      work(std::true_type(), in, tile++);
+      in = next;
+    }
+    for (; tile < t.tiles; ++tile) {   // at most once, unless rows lie far apart
+      if (tile > t.full) load(std::false_type(), in, tile);
+      work(std::false_type(), in, tile);
+    }
   }
-  if (tile < full) {
-    load_tile<false, AL>(next, fx, fg, first + full * tile_rows);
-    work(std::true_type(), in, tile);
-    in = next;
-  }
-  if (w.seqs > 1 || full * tile_rows < t.n) work(std::false_type(), in, full);
-  if (t.on && b.steps) zero_behind<AL, V>(y, b, t, w.per);
+  // the state behind the last row, from the thread that walked it: the very value that y rounds
+  const int lead = t.n > 0 ? (t.n - 1) / R % w.per : 0;
+  if (t.on && q.last && t.sub == lead && (t.n > 0 ? t.tile < t.tiles && t.tiles * w.per * R >= t.n : t.piece == 0))
+#pragma unroll
+    for (int v = 0; v < V; ++v) q.last[end + v] = t.n > 0 ? h[v] : carry[v];
+  if (t.on && b.steps) zero_behind<AL, V>(y, b, w, t);
 }
 
 // Gradient.  With e_t = a_t delta_t, delta_t = gy_t + e_{t+1}, the way back is a composition of maps e -> A (gy + e) with the
@@ -284,33 +428,29 @@ __global__ void __launch_bounds__(kSeqThreads, 2) gated_scan_backward_kernel(con
                                                                              const Rows<const T> g, const Rows<const T> gy, const Rows<T> gx,
                                                                              const Rows<T> gg, const ScanPtrs q) {
   constexpr int R = kSlotRows;
-  __shared__ float maps[2][3][kSeqThreads * V];
-  const Seat t = seat_of<V>(b, w, blockIdx.x, blockIdx.y);
+  alignas(8) __shared__ float maps[2][3][kSeqThreads * V];
+  const Seat t = seat_of<V>(b, w);
+  if (!t.there) return;
   const bool no_gy = !gy.p;
-  const Source<T> fx = source_of(x, b, t), fg = source_of(g, b, t), fd = no_gy ? fx : source_of(gy, b, t);
-  const int64_t gxs = b.reverse ? -gx.rs : gx.rs, ggs = b.reverse ? -gg.rs : gg.rs;
-  T* const gxp = row_base(gx, b, t.u, t.s) + t.col;
-  T* const ggp = row_base(gg, b, t.u, t.s) + t.col;
-  const int tile_rows = w.per * R;
+  const Lane<const T> fx = lane_of<V>(x, b, w, t), fg = lane_of<V>(g, b, w, t), fd = no_gy ? fx : lane_of<V>(gy, b, w, t);
+  const Lane<T> fgx = lane_of<V>(gx, b, w, t), fgg = lane_of<V>(gg, b, w, t);
   const int64_t end = t.u * b.ncol + t.col;
   float carry[V] = {};
   if (t.on && q.glast)
 #pragma unroll
     for (int v = 0; v < V; ++v) carry[v] = q.glast[end + v];
   const int64_t ck_step = t.n > 0 ? b.ncol : 0;
-  const float* const ck = t.n > 0 ? q.ckpt + checkpoint_row(b, t, tile_rows) * b.ncol + t.col : q.ckpt;
+  const float* const ck = t.n > 0 ? q.ckpt + checkpoint_row(b, t, w.per * R) * b.ncol + t.col : q.ckpt;
 
   auto load = [&](auto full, ScanGradRows<T, V>& r, int tile) {
-    const int t0 = (tile * w.per + t.sub) * R;
-    load_rows<full(), AL>(r.x, fx, t0);
-    load_rows<full(), AL>(r.g, fg, t0);
-    load_rows<full(), AL>(r.d, fd, t0);
+    load_rows<full(), AL>(r.x, fx, t, w, tile);
+    load_rows<full(), AL>(r.g, fg, t, w, tile);
+    load_rows<full(), AL>(r.d, fd, t, w, tile);
     load_pack<false>(r.h, ck + tile * ck_step);
   };
   auto work = [&](auto full, const ScanGradRows<T, V>& in, int tile) {
     constexpr bool FULL = full();
-    const int t0 = (tile * w.per + t.sub) * R;
-    const int k = FULL ? R : min(max(t.n - t0, 0), R);
+    const int k = FULL ? R : min(max(t.n - (tile * w.per + t.sub) * R, 0), R);
     float a[R][V], na[R][V], A[V], X[V], E[V], h[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) A[v] = 1.0f, X[v] = 0.0f, E[v] = 0.0f, h[v] = in.h.v[v];
@@ -362,10 +502,8 @@ __global__ void __launch_bounds__(kSeqThreads, 2) gated_scan_backward_kernel(con
           hp[r][v] = h[v];
           h[v] = fmaf(a[r][v], h[v], FULL || r < k ? na[r][v] * (float)in.x[r].v[v] : 0.0f);
         }
-      T* ox = gxp + (t0 + R - 1) * gxs;
-      T* og = ggp + (t0 + R - 1) * ggs;
 #pragma unroll
-      for (int r = R - 1; r >= 0; --r, ox -= gxs, og -= ggs) {
+      for (int r = R - 1; r >= 0; --r) {
         float dx[V], dg[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -375,35 +513,40 @@ __global__ void __launch_bounds__(kSeqThreads, 2) gated_scan_backward_kernel(con
           dg[v] = SIG ? e[v] * na[r][v] * (hp[r][v] - (float)in.x[r].v[v]) : d * hp[r][v];
         }
         if (FULL || r < k) {
-          store_pack<AL, V>(ox, dx);
-          store_pack<AL, V>(og, dg);
+          store_pack<AL, V>(row_at<FULL>(fgx, t, w, tile, r), dx);
+          store_pack<AL, V>(row_at<FULL>(fgg, t, w, tile, r), dg);
         }
       }
     }
   };
 
-  ScanGradRows<T, V> in, next;
-  const int full = w.seqs > 1 ? 0 : t.n / tile_rows;
-  if (x.p && (w.seqs > 1 || full * tile_rows < t.n)) {
-    load(std::false_type(), in, full);
-    work(std::false_type(), in, full);
-  }
-  if (full > 0) {
-    load(std::true_type(), in, full - 1);
-    int tile = full - 1;
-    for (; tile > 0; --tile) {
-      load(std::true_type(), next, tile - 1);
-      work(std::true_type(), in, tile);
-      in = next;
+  if (x.p && t.tile < t.tiles) {   // the same for the whole workgroup
+    ScanGradRows<T, V> in, next;
+    if (w.pieces > 1) {
+      const int piece_rows = w.piece_tiles * w.per * R, pieces = (t.n + piece_rows - 1) / piece_rows;   // of this sequence
+      enter_piece(carry, q.maps + (t.u * w.pieces + pieces - 1) * b.ncol + t.col, -(int64_t)b.ncol, pieces - 1 - t.piece, w, t, (float2*)maps);
     }
-    work(std::true_type(), in, 0);
+    int tile = t.tiles - 1;
+    for (; tile >= t.full; --tile) {   // at most once, unless rows lie far apart
+      load(std::false_type(), in, tile);
+      work(std::false_type(), in, tile);
+    }
+    if (tile >= t.tile) {
+      load(std::true_type(), in, tile);
+      for (; tile > t.tile; --tile) {
+        load(std::true_type(), next, tile - 1);
+        work(std::true_type(), in, tile);
+        in = next;
+      }
+      work(std::true_type(), in, tile);
+    }
   }
-  if (t.on && q.gh0 && t.sub == 0)
+  if (t.on && q.gh0 && t.sub == 0 && t.piece == 0)
 #pragma unroll
     for (int v = 0; v < V; ++v) q.gh0[end + v] = carry[v];
   if (t.on && b.steps) {
-    zero_behind<AL, V>(gx, b, t, w.per);
-    zero_behind<AL, V>(gg, b, t, w.per);
+    zero_behind<AL, V>(gx, b, w, t);
+    zero_behind<AL, V>(gg, b, w, t);
   }
 }
 

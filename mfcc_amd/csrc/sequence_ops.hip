@@ -12,6 +12,7 @@ using mfcc::Rows;
 namespace {
 
 constexpr int64_t kMaxColumns = 1 << 20;
+constexpr int64_t kMaxSeqs = 1 << 24;
 constexpr int64_t kMaxRows = 1 << 30;  // of one sequence: row numbers inside it are 32-bit
 
 // The geometry of a call, checked once: 0 or a negative error code.
@@ -23,8 +24,8 @@ int shape_of(const char* who, const mfcc_layout* layout, int64_t n_seq, int64_t 
   if (ncol < 1 || ncol > kMaxColumns) return fail(MFCC_ERR_INVALID, "%s: ncol=%d outside 1..%lld", who, ncol, (long long)kMaxColumns);
   if (time_steps < 0 || time_steps > INT32_MAX) return fail(MFCC_ERR_INVALID, "%s: time_steps=%lld outside 0..2^31-1", who, (long long)time_steps);
   if (layout) n_seq = layout->n_utts;
-  if (n_seq < 0 || n_seq > INT32_MAX) return fail(MFCC_ERR_INVALID, "%s: %lld sequences outside 0..2^31-1", who, (long long)n_seq);
-  out->b = Batch{layout ? layout->d_frame_off : nullptr, n_seq, time_steps, ncol, reverse};
+  if (n_seq < 0 || n_seq > kMaxSeqs) return fail(MFCC_ERR_INVALID, "%s: %lld sequences outside 0..2^24", who, (long long)n_seq);
+  out->b = Batch{layout ? layout->d_frame_off : nullptr, layout ? layout->d_order : nullptr, n_seq, time_steps, ncol, reverse};
   out->longest = layout ? (time_steps ? std::min(layout->longest, time_steps) : layout->longest) : time_steps;
   out->rows = time_steps || !layout ? n_seq * time_steps : layout->total_frames;
   if (out->longest > kMaxRows) return fail(MFCC_ERR_UNSUPPORTED, "%s: a sequence of more than 2^30 rows", who);
@@ -47,6 +48,12 @@ int check_rows(const char* who, const char* name, const mfcc_rows* r, const Shap
   return MFCC_OK;
 }
 
+// Where workgroups of one sequence are fewer than the compute units, sequences of many tiles are cut into pieces, and others spread over
+// narrower column blocks.  Measured with 512 columns of bfloat16, forward (training step): one sequence of 512 rows (8 tiles)
+// 11.1 (31.6) us whole, 12.8 (27.8) in pieces of 2 tiles; of 1024 rows 18.8 (56.6) and 13.3 (29.0), of 8192 rows 124 (396) and
+// 17.1 (38.8).  32 sequences of up to 700 rows (11 tiles, 4 pieces would fill the card) 18.9 us whole, 28 in pieces.
+constexpr int64_t kFewBlocks = 256, kManyTiles = 10, kManyPieces = 5, kTargetBlocks = 512, kPieceTiles = 2;
+
 // How workgroups divide sequences, columns and time.  It depends on the shape of the batch alone, so that the backward
 // pass finds its checkpoints whatever the alignment of its arrays.
 struct Grid {
@@ -57,24 +64,53 @@ struct Grid {
 Grid grid_of(const Shape& s) {
   Grid g;
   g.v = s.b.ncol % 2 ? 1 : 2;   // values of a row that a thread takes at once
-  const int rows = mfcc::kSlotRows;
   g.w.groups = s.b.ncol / g.v;
-  // column blocks of at most a wave's width, equally wide
-  const int nb = (g.w.groups + 63) / 64;
-  g.w.cb = (g.w.groups + nb - 1) / nb;
-  // slots of time: as many as the threads give, at most 64 (each thread composes the maps of all of them), and no more
-  // than the longest sequence fills; what is left over takes further sequences
-  const int slots = mfcc::kSeqThreads / g.w.cb;
-  const int64_t need = std::max<int64_t>(1, (s.longest + rows - 1) / rows);
-  g.w.per = (int32_t)std::min<int64_t>(std::min(slots, 64), need);
-  g.w.seqs = need <= g.w.per ? slots / g.w.per : 1;
-  g.tile_rows = g.w.per * rows;
-  g.blocks = dim3(blocks_for(s.b.n_seq, g.w.seqs), (unsigned)nb);
+  g.w.pieces = 1;
+  g.w.near = 1;
+  // column blocks of at most `wide` groups, equally wide; slots of time: as many as the threads give, at most 64 (each thread
+  // composes the maps of all of them), and no more than the longest sequence fills; what is left over takes further sequences
+  auto split = [&](int wide) {
+    g.w.column_blocks = (g.w.groups + wide - 1) / wide;
+    g.w.cb = (g.w.groups + g.w.column_blocks - 1) / g.w.column_blocks;
+    const int slots = mfcc::kSeqThreads / g.w.cb;
+    const int64_t need = std::max<int64_t>(1, (s.longest + mfcc::kSlotRows - 1) / mfcc::kSlotRows);
+    g.w.per = (int32_t)std::min<int64_t>(std::min(slots, 64), need);
+    g.w.seqs = need <= g.w.per ? slots / g.w.per : 1;
+    g.tile_rows = g.w.per * mfcc::kSlotRows;
+    g.w.blocks = (int32_t)blocks_for(s.b.n_seq, g.w.seqs);
+    g.w.piece_tiles = (int32_t)std::max<int64_t>((s.longest + g.tile_rows - 1) / g.tile_rows, 1);
+  };
+  split(64);   // a wave to a row
+  const int64_t blocks = (int64_t)g.w.blocks * g.w.column_blocks, tiles = g.w.piece_tiles;
+  if (g.w.seqs == 1 && blocks > 0 && blocks < kFewBlocks) {
+    const int64_t want = std::min((kTargetBlocks + blocks - 1) / blocks, tiles / kPieceTiles);
+    if (tiles >= kManyTiles && want >= kManyPieces) {
+      g.w.piece_tiles = (int32_t)((tiles + want - 1) / want);
+      g.w.pieces = (int32_t)((tiles + g.w.piece_tiles - 1) / g.w.piece_tiles);
+      g.w.blocks *= g.w.pieces;
+    } else {
+      split(32);   // twice the workgroups, of half the tiles (32 sequences of up to 700 rows: 23.6 -> 18.9 us)
+    }
+  }
+  g.blocks = dim3((unsigned)((g.w.blocks + 7) / 8 * 8 * g.w.column_blocks));
   return g;
+}
+
+int check_grid(const char* who, const Shape& s, const Grid& g, const void* workspace) {
+  if ((s.b.n_seq + 7) * g.w.column_blocks > INT32_MAX)
+    return fail(MFCC_ERR_UNSUPPORTED, "%s: %lld sequences of %d columns are more than one launch covers", who, (long long)s.b.n_seq, s.b.ncol);
+  if (g.w.pieces > 1 && (!workspace || ((uintptr_t)workspace & 15)))
+    return fail(MFCC_ERR_INVALID, "%s: this shape needs a 16-byte aligned workspace (mfcc_sequence_workspace)", who);
+  return MFCC_OK;
 }
 
 bool aligned(const mfcc_rows* r, const Shape& s, int v, size_t size) {
   return !r || (((uintptr_t)r->data % (v * size)) == 0 && r->row_stride % v == 0 && (s.b.steps == 0 || r->seq_stride % v == 0));
+}
+
+// Offsets inside a tile are 32-bit numbers of bytes where that is enough.
+bool near(const mfcc_rows* r, const Grid& c, const Shape& s, size_t size) {
+  return !r || (c.tile_rows * (double)r->row_stride + s.b.ncol) * size < 4294967296.0;
 }
 
 // f(type's zero, number of values, aligned) for the row type, the values a thread takes and the alignment of the arrays
@@ -115,7 +151,8 @@ int64_t mfcc_sequence_workspace(const mfcc_layout* layout, int64_t n_seq, int64_
   Shape s;
   if (const int rc = shape_of("mfcc_sequence_workspace", layout, n_seq, time_steps, ncol, 0, &s)) return rc;
   if (rows_dtype < 0 || rows_dtype > MFCC_ROWS_F16) return bad_dtype("mfcc_sequence_workspace", rows_dtype);
-  return 0;
+  const Grid g = grid_of(s);
+  return g.w.pieces > 1 ? s.b.n_seq * g.w.pieces * ncol * (int64_t)sizeof(float2) : 0;
 }
 
 int mfcc_gated_scan(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype, int32_t form,
@@ -130,12 +167,20 @@ int mfcc_gated_scan(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps
   if (const int rc = check_rows(who, "y", y, s, true)) return rc;
   if (rows_dtype < 0 || rows_dtype > MFCC_ROWS_F16) return bad_dtype(who, rows_dtype);
   if (s.b.n_seq == 0) return MFCC_OK;
-  const mfcc::ScanPtrs q{h0, nullptr, last, checkpoints, nullptr};
-  const Grid c = grid_of(s);
+  Grid c = grid_of(s);
+  if (const int rc = check_grid(who, s, c, workspace)) return rc;
+  const mfcc::ScanPtrs q{h0, nullptr, last, checkpoints, nullptr, (float2*)workspace};
   const size_t size = rows_dtype == MFCC_ROWS_F32 ? 4 : 2;
   const bool al = aligned(x, s, c.v, size) && aligned(gate, s, c.v, size) && aligned(y, s, c.v, size);
+  c.w.near = near(x, c, s, size) && near(gate, c, s, size) && near(y, c, s, size);
   dispatch(rows_dtype, c.v, al, [&](auto zero, auto v, auto al) {
     using T = decltype(zero);
+    if (c.w.pieces > 1) {
+      auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_pieces_kernel<T, v(), al(), true, false>
+                                         : mfcc::gated_scan_pieces_kernel<T, v(), al(), false, false>;
+      hipLaunchKernelGGL(k, c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const T>(x, s),
+                         rows_of<const T>(gate, s), q);
+    }
     auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_kernel<T, v(), al(), true> : mfcc::gated_scan_kernel<T, v(), al(), false>;
     hipLaunchKernelGGL(k, c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const T>(x, s), rows_of<const T>(gate, s),
                        rows_of<T>(y, s), q);
@@ -161,13 +206,21 @@ int mfcc_gated_scan_backward(const mfcc_layout* layout, int64_t n_seq, int64_t t
   if (!checkpoints && s.rows > 0) return fail(MFCC_ERR_INVALID, "%s: checkpoints is null", who);
   if (rows_dtype < 0 || rows_dtype > MFCC_ROWS_F16) return bad_dtype(who, rows_dtype);
   if (s.b.n_seq == 0) return MFCC_OK;
-  const mfcc::ScanPtrs q{nullptr, grad_last, nullptr, const_cast<float*>(checkpoints), grad_h0};
-  const Grid c = grid_of(s);
+  Grid c = grid_of(s);
+  if (const int rc = check_grid(who, s, c, workspace)) return rc;
+  const mfcc::ScanPtrs q{nullptr, grad_last, nullptr, const_cast<float*>(checkpoints), grad_h0, (float2*)workspace};
   const size_t size = rows_dtype == MFCC_ROWS_F32 ? 4 : 2;
   const bool al = aligned(x, s, c.v, size) && aligned(gate, s, c.v, size) && aligned(grad_y, s, c.v, size) && aligned(grad_x, s, c.v, size) &&
             aligned(grad_gate, s, c.v, size);
+  c.w.near = near(x, c, s, size) && near(gate, c, s, size) && near(grad_y, c, s, size) && near(grad_x, c, s, size) && near(grad_gate, c, s, size);
   dispatch(rows_dtype, c.v, al, [&](auto zero, auto v, auto al) {
     using T = decltype(zero);
+    if (c.w.pieces > 1) {
+      auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_pieces_kernel<T, v(), al(), true, true>
+                                         : mfcc::gated_scan_pieces_kernel<T, v(), al(), false, true>;
+      hipLaunchKernelGGL(k, c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const T>(grad_y, s),
+                         rows_of<const T>(gate, s), q);
+    }
     auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_backward_kernel<T, v(), al(), true> : mfcc::gated_scan_backward_kernel<T, v(), al(), false>;
     hipLaunchKernelGGL(k, c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const T>(x, s), rows_of<const T>(gate, s),
                        rows_of<const T>(grad_y, s), rows_of<T>(grad_x, s), rows_of<T>(grad_gate, s), q);
