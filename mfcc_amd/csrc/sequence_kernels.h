@@ -568,39 +568,266 @@ __global__ void __launch_bounds__(256) gated_scan_step_kernel(int64_t n, int nco
   y[u * y_ld + c] = (T)h;
 }
 
-// Simplest form: one thread walks one column.  The statistics are kept in 64 bits: at a fixed point of w the roundings
-// of 32 bits all have one sign (7e-6 of w off after 20000 rows at decay 0.995), and a cumulative mean of 20000 rows
-// collects 20 units in the last place.
-template <typename T>
-__global__ void __launch_bounds__(256) running_norm_kernel(const Batch b, const Rows<const float> x, const Rows<T> y, double decay, float eps,
-                                                           int center_only, const float* state_in, float* state_out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= b.n_seq * b.ncol) return;
-  const int64_t u = i / b.ncol;
-  const int c = (int)(i % b.ncol);
-  const Span s = span_of(b, u);
-  const float* xp = row_base(x, b, u, s) + c;
-  T* yp = row_base(y, b, u, s) + c;
-  const int64_t st = u * (1 + 2 * (int64_t)b.ncol);
-  double w = 0, m = 0, q = 0;
-  if (state_in) w = state_in[st], m = state_in[st + 1 + c], q = state_in[st + 1 + b.ncol + c];
-  for (int64_t t = 0; t < s.n; ++t) {
-    const double v = xp[t * x.rs], d = v - m;
-    w = fma(decay, w, 1.0);
-    const double inv = 1.0 / w;
-    m = fma(d, inv, m);
-    const double e = v - m;
-    q = fma(decay, q, d * e);
-    yp[t * y.rs] = (T)(center_only ? (float)e : (float)e * rsqrtf((float)(q * inv) + eps));
-  }
-  if (state_out) {
-    if (c == 0) state_out[st] = (float)w;  // every column carries the same weight
-    state_out[st + 1 + c] = (float)m;
-    state_out[st + 1 + b.ncol + c] = (float)q;
-  }
-  for (int64_t t = s.n; t < b.steps; ++t) y.p[u * y.ss + t * y.rs + c] = (T)0.0f;
+// ---- running normalisation ---------------------------------------------------------------------------
+// A run of k rows is (m, q): its mean and its sum of squared deviations under the weights decay^(k-1) .. 1, whose sum is
+// g(k) = 1 + decay + .. + decay^(k-1). A run behind one of weight w joins to
+//   w' = decay^k w + g,  f = g / w',  m' = m + (m_run - m) f,  q' = decay^k q + q_run + (m_run - m)^2 decay^k w f,
+// without a difference of squares. The weights depend on the row number alone: they are carried in 64 bits from tile to tile (at the fixed
+// point of w the roundings of 32 bits have one sign: 7e-6 of w off after 20000 rows at decay 0.995), and f and decay^k w f are
+// computed once per slot. The mean that enters a tile is carried in 64 bits and the tile composes 32-bit deviations from it: a
+// cumulative mean of n rows would otherwise collect sqrt(n) / 4 units in the last place.
+// Bound: HBM, one value read and one written; 25 operations a value.
+struct NormArgs {
+  double decay, log_decay;      // log_decay = log1p(decay - 1)
+  double slot_decay, slot_grown, tile_decay, tile_grown;   // decay^k and g(k) of a slot and of a tile
+  float eps, inv_grown[kSlotRows];   // 1 / g(1) .. 1 / g(R)
+  int center_only;
+  const float* state_in;
+  float* state_out;
+  float2* runs;                 // [sequence][piece][column] (m, q) where sequences are cut into pieces
+};
+
+// decay^k and g(k)
+__device__ inline void weights_of(const NormArgs& a, double k, double& decayed, double& grown) {
+  const double em = expm1(k * a.log_decay);
+  decayed = 1.0 + em;
+  grown = a.decay == 1.0 ? k : em / (a.decay - 1.0);
 }
 
+// (m, q) of k rows, one after the other.
+template <int V, int N, bool ALL>
+__device__ inline void norm_run(float (&m)[V], float (&q)[V], float& w, float decay, const Pack<float, V> (&x)[N], int k, const float* inv) {
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    w = ALL || r < k ? fmaf(decay, w, 1.0f) : w;
+    const float f = inv ? inv[r] : __builtin_amdgcn_rcpf(w);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float d = x[r].v[v] - m[v], mn = fmaf(d, f, m[v]), qn = fmaf(d, x[r].v[v] - mn, decay * q[v]);
+      m[v] = ALL || r < k ? mn : m[v];
+      q[v] = ALL || r < k ? qn : q[v];
+    }
+  }
+}
+
+// (w, m, q) and behind it (g, m2, q2) after `decayed` of the first is left.
+__device__ inline void norm_join(float& w, float& m, float& q, float decayed, float g, float m2, float q2) {
+  const float old = decayed * w, sum = old + g, f = old > 0.0f ? g * __builtin_amdgcn_rcpf(sum) : 1.0f, d = m2 - m;   // g > 0
+  w = sum;
+  m = fmaf(d, f, m);
+  q = fmaf(decayed, q, fmaf(d * d, old * f, q2));
+}
+
+template <int V, bool AL>
+__global__ void __launch_bounds__(kSeqThreads, 4) running_norm_pieces_kernel(const Batch b, const Split w, const Rows<const float> x, const NormArgs a) {
+  constexpr int R = kSlotRows;
+  __shared__ float2 runs[kSeqThreads * V];
+  const Seat t = seat_of<V>(b, w);
+  if (!t.there || t.tile >= t.tiles || !x.p) return;   // the same for the whole workgroup
+  const Lane<const float> fx = lane_of<V>(x, b, w, t);
+  const int run = w.piece_tiles * R, first = t.tile * w.per * R, begin = first + t.sub * run, len = min(max(t.n - begin, 0), run);
+  auto load = [&](Pack<float, V>(&r)[R], int at) {
+    const float* p = fx.p + min(begin + at, t.n - 1) * fx.rs;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      load_pack<AL>(r[i], p);
+      p += begin + at + i < t.n - 1 ? fx.rs : 0;
+    }
+  };
+  Pack<float, V> in[R], next[R];
+  float m[V] = {}, q[V] = {}, sum = 0.0f;
+  load(in, 0);
+  for (int i = 0; i < len; i += R) {
+    load(next, i + R);
+    norm_run<V, R, false>(m, q, sum, (float)a.decay, in, len - i, nullptr);
+#pragma unroll
+    for (int r = 0; r < R; ++r) in[r] = next[r];
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) runs[(t.slot * V + v) * w.cb + t.cg] = make_float2(m[v], q[v]);
+  __syncthreads();
+  if (t.sub == 0) {
+    double l, g;
+    weights_of(a, run, l, g);
+    float ws = 0.0f, ms[V] = {}, qs[V] = {};
+    for (int s = 0; s < w.per; ++s) {
+      const int k = min(max(t.n - first - s * run, 0), run);
+      if (k == 0) break;
+      if (k < run) weights_of(a, k, l, g);
+      float wn = ws;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float2 e = runs[(s * V + v) * w.cb + t.cg];
+        wn = ws;
+        norm_join(wn, ms[v], qs[v], (float)l, (float)g, e.x, e.y);
+      }
+      ws = wn;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) a.runs[(t.u * w.pieces + t.piece) * b.ncol + t.col + v] = make_float2(ms[v], qs[v]);
+  }
+}
+
+template <typename T, int V, bool AL>
+__global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batch b, const Split w, const Rows<const float> x, const Rows<T> y,
+                                                                      const NormArgs a) {
+  constexpr int R = kSlotRows;
+  __shared__ float2 runs[2][kSeqThreads * V];
+  __shared__ float4 joins[2][kSeqThreads];   // of every slot: f, decay^k w f, decay^k
+  const Seat t = seat_of<V>(b, w);
+  if (!t.there) return;
+  const Lane<const float> fx = lane_of<V>(x, b, w, t);
+  const Lane<T> fy = lane_of<V>(y, b, w, t);
+  const float decay = (float)a.decay;
+  const int64_t state = t.u * (1 + 2 * (int64_t)b.ncol);
+  // decay^k and g(k) of the rows of a tile before the thread's slot
+  double before_decay = 1.0, before_grown = 0.0;
+  for (int s = 0; s < t.sub; ++s) before_decay *= a.slot_decay, before_grown = fma(a.slot_decay, before_grown, a.slot_grown);
+  double weight = 0.0, mean[V] = {};   // that enter the tile
+  float square[V] = {}, m[V] = {}, q[V] = {};
+  if (t.on && a.state_in) {
+    weight = a.state_in[state];
+#pragma unroll
+    for (int v = 0; v < V; ++v) mean[v] = a.state_in[state + 1 + t.col + v], square[v] = a.state_in[state + 1 + b.ncol + t.col + v];
+  }
+
+  auto work = [&](auto full, const Pack<float, V>(&in)[R], int tile) {
+    constexpr bool FULL = full();
+    const int k = FULL ? R : min(max(t.n - (tile * w.per + t.sub) * R, 0), R);
+    float ws = (float)fma(before_decay, weight, before_grown);
+    float base[V], off[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) base[v] = (float)mean[v], off[v] = (float)(mean[v] - base[v]);
+    if (w.per > 1) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) m[v] = 0.0f, q[v] = 0.0f;
+      float none = 0.0f;
+      norm_run<V, R, FULL>(m, q, none, decay, in, k, a.inv_grown);
+      float l = (float)a.slot_decay, g = (float)a.slot_grown;
+      if (!FULL && k < R) {
+        l = 1.0f, g = 0.0f;
+        for (int r = 0; r < k; ++r) l *= decay, g = fmaf(decay, g, 1.0f);
+      }
+      const float old = l * ws, f = g == 0.0f ? 0.0f : old > 0.0f ? g * __builtin_amdgcn_rcpf(old + g) : 1.0f;   // a first run is its own mean
+      float2* const e = runs[tile & 1];
+      float4* const j = joins[tile & 1];
+#pragma unroll
+      for (int v = 0; v < V; ++v) e[(t.slot * V + v) * w.cb + t.cg] = make_float2(m[v], q[v]);
+      if (t.cg == 0) j[t.slot] = make_float4(f, old * f, l, 0.0f);
+      __syncthreads();
+      const int first = t.slot - t.sub;
+#pragma unroll 2
+      for (int s = 0; s < w.per; ++s) {
+        const float4 p = j[first + s];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float2 r = e[((first + s) * V + v) * w.cb + t.cg];
+          m[v] = s == t.sub ? off[v] : m[v];
+          q[v] = s == t.sub ? square[v] : q[v];
+          const float d = r.x - base[v] - off[v];
+          off[v] = fmaf(d, p.x, off[v]);
+          square[v] = fmaf(p.z, square[v], fmaf(d * d, p.y, r.y));
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        mean[v] = (double)base[v] + off[v];
+        m[v] += base[v];
+      }
+      weight = fma(a.tile_decay, weight, a.tile_grown);   // behind a last tile with missing rows it is not used
+    } else {
+      __syncthreads();   // doubles have read their rows: y may be x
+#pragma unroll
+      for (int v = 0; v < V; ++v) m[v] = base[v], q[v] = square[v];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      ws = fmaf(decay, ws, 1.0f);
+      const float f = __builtin_amdgcn_rcpf(ws);
+      float o[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float d = in[r].v[v] - m[v], mn = fmaf(d, f, m[v]), c = in[r].v[v] - mn, qn = fmaf(d, c, decay * q[v]);
+        o[v] = a.center_only ? c : c * __builtin_amdgcn_rsqf(fmaf(qn, f, a.eps));
+        m[v] = FULL || r < k ? mn : m[v];
+        q[v] = FULL || r < k ? qn : q[v];
+      }
+      if (FULL || r < k) store_pack<AL, V>(row_at<FULL>(fy, t, w, tile, r), o);
+    }
+  };
+
+  if (x.p && t.tile < t.tiles) {   // the same for the whole workgroup
+    Pack<float, V> in[R], next[R];
+    int tile = t.tile;
+    load_rows<false, AL>(in, fx, t, w, tile);
+    if (t.piece > 0) {
+      // the pieces before this one: each slot joins a run of them, the slots meet in LDS
+      double l, g, lr, gr;
+      weights_of(a, w.piece_tiles * w.per * R, l, g);
+      const int run = (t.piece + w.per - 1) / w.per, lo = t.sub * run, hi = min(lo + run, t.piece);
+      const float2* p = a.runs + (t.u * w.pieces + lo) * b.ncol + t.col;
+      float sum = 0.0f;
+#pragma unroll 8
+      for (int i = lo; i < hi; ++i, p += b.ncol) {
+        float wn = sum;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          wn = sum;
+          norm_join(wn, m[v], q[v], (float)l, (float)g, p[v].x, p[v].y);
+        }
+        sum = wn;
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) runs[0][(t.slot * V + v) * w.cb + t.cg] = make_float2(m[v], q[v]);
+      __syncthreads();
+      weights_of(a, (double)run * w.piece_tiles * w.per * R, lr, gr);
+      for (int s = 0; s < w.per && s * run < t.piece; ++s) {
+        if (t.piece - s * run < run) weights_of(a, (double)(t.piece - s * run) * w.piece_tiles * w.per * R, lr, gr);
+        const double old = lr * weight, f = gr / (old + gr);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float2 e = runs[0][(s * V + v) * w.cb + t.cg];
+          const double d = e.x - mean[v];
+          mean[v] = fma(d, f, mean[v]);
+          square[v] = (float)(lr * square[v] + e.y + d * d * old * f);
+        }
+        weight = old + gr;
+      }
+      __syncthreads();
+    }
+    for (; tile + 1 < t.full; ++tile) {
+      load_rows<true, AL>(next, fx, t, w, tile + 1);
+      work(std::true_type(), in, tile);
+#pragma unroll
+      for (int r = 0; r < R; ++r) in[r] = next[r];
+    }
+    if (tile < t.full) {
+      if (t.full < t.tiles) load_rows<false, AL>(next, fx, t, w, t.full);
+      work(std::true_type(), in, tile++);
+#pragma unroll
+      for (int r = 0; r < R; ++r) in[r] = next[r];
+    }
+    for (; tile < t.tiles; ++tile) {   // at most once, unless rows lie far apart
+      if (tile > t.full) load_rows<false, AL>(in, fx, t, w, tile);
+      work(std::false_type(), in, tile);
+    }
+  }
+  // the state behind the last row, from the thread that walked it
+  const int lead = t.n > 0 ? (t.n - 1) / R % w.per : 0;
+  if (t.on && a.state_out && t.sub == lead && (t.n > 0 ? t.tile < t.tiles && t.tiles * w.per * R >= t.n : t.piece == 0)) {
+    double l, g;
+    weights_of(a, t.n, l, g);
+    if (t.col == 0) a.state_out[state] = (float)(l * (a.state_in ? (double)a.state_in[state] : 0.0) + g);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      a.state_out[state + 1 + t.col + v] = t.n > 0 ? m[v] : (float)mean[v];
+      a.state_out[state + 1 + b.ncol + t.col + v] = t.n > 0 ? q[v] : square[v];
+    }
+  }
+  if (t.on && b.steps) zero_behind<AL, V>(y, b, w, t);
+}
+
+// ---- dropout --------------------------------------------------------------------------------------------
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011): two 32 x 32 -> 64 bit
 // products a round, the key raised by two Weyl constants.
 __device__ inline uint4 philox4x32_10(uint64_t block, uint64_t step, uint64_t seed) {
@@ -618,38 +845,103 @@ __device__ inline uint4 philox4x32_10(uint64_t block, uint64_t step, uint64_t se
   }
   return make_uint4(c0, c1, c2, c3);
 }
-__device__ inline uint32_t philox_field(const uint4& w, int k) {
-  const uint32_t v = (k >> 1) == 0 ? w.x : (k >> 1) == 1 ? w.y : (k >> 1) == 2 ? w.z : w.w;
-  return k & 1 ? v >> 16 : v & 0xFFFFu;
+// Bit k of the result: field k of the block is below the threshold, its element dropped.
+__device__ inline uint32_t philox_dropped(uint64_t block, uint64_t step, uint64_t seed, uint32_t threshold) {
+  const uint4 w = philox4x32_10(block, step, seed);
+  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+  uint32_t bits = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) bits |= ((v[k] & 0xFFFFu) < threshold ? 1u : 0u) << (2 * k) | ((v[k] >> 16) < threshold ? 2u : 0u) << (2 * k);
+  return bits;
 }
 
-// Simplest form: one thread per element.
-template <typename T>
-__global__ void __launch_bounds__(256) feature_dropout_kernel(const Batch b, int64_t n_rows, int per, uint32_t threshold, float scale,
-                                                              uint64_t seed, uint64_t step, const int64_t* step_device,
-                                                              const Rows<const T> x, const Rows<T> y) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n_rows * b.ncol) return;
-  const int64_t r = i / b.ncol;
-  const int c = (int)(i % b.ncol);
-  int64_t u = 0, t = r;
-  if (b.steps) {
-    u = r / b.steps;
-    t = r % b.steps;
-  } else if (per == 2) {  // the last u with off[u] <= r
-    int64_t lo = 0, hi = b.n_seq;
-    while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) / 2;
-      if (b.off[mid] <= r) lo = mid; else hi = mid;
+struct Dropout {
+  uint64_t seed, step;
+  const int64_t* step_device;
+  uint32_t threshold;
+  float scale;
+  __device__ uint64_t at() const { return step_device ? (uint64_t)*step_device : step; }
+};
+
+// per = element: a thread takes the 8 consecutive elements of one block. FLAT: rows back to back in both arrays and 16-byte
+// aligned, an element is its number. Otherwise (row, column) of the first one by division, then step by step.
+// Bound: HBM, read once and written once (20000 x 4369 bfloat16, both passes: see the table of measurements); the 20 wide products
+// of a block are shared by 8 elements.
+template <typename T, bool FLAT>
+__global__ void __launch_bounds__(256) dropout_element_kernel(const Batch b, int64_t n_rows, const Dropout d, const Rows<const T> x,
+                                                              const Rows<T> y) {
+  const int64_t block = (int64_t)blockIdx.x * 256 + threadIdx.x, total = n_rows * b.ncol, e0 = block * 8;
+  if (e0 >= total) return;
+  const uint32_t gone = philox_dropped((uint64_t)block, d.at(), d.seed, d.threshold);
+  if (FLAT && e0 + 8 <= total) {
+    constexpr int V = 16 / sizeof(T);
+    Pack<T, V> r[8 / V];
+#pragma unroll
+    for (int i = 0; i < 8 / V; ++i) r[i] = *(const Pack<T, V>*)(x.p + e0 + i * V);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      T& v = r[i / V].v[i % V];
+      v = gone >> i & 1 ? (T)0.0f : (T)((float)v * d.scale);
     }
-    u = lo;
+#pragma unroll
+    for (int i = 0; i < 8 / V; ++i) *(Pack<T, V>*)(y.p + e0 + i * V) = r[i];
+    return;
   }
-  const uint64_t e = per == 0 ? (uint64_t)i : per == 1 ? (uint64_t)r : (uint64_t)u * ((b.ncol + 7) / 8 * 8) + c;
-  const uint64_t st = step_device ? (uint64_t)*step_device : step;
-  const uint32_t f = philox_field(philox4x32_10(e >> 3, st, seed), (int)(e & 7));
-  const int64_t at = b.steps ? u * x.ss + t * x.rs + c : r * x.rs + c;
-  const int64_t to = b.steps ? u * y.ss + t * y.rs + c : r * y.rs + c;
-  y.p[to] = f < threshold ? (T)0.0f : (T)((float)x.p[at] * scale);
+  const int64_t row = e0 / b.ncol;
+  int64_t c = e0 - row * b.ncol, u = b.steps ? row / b.steps : 0, t = row - u * b.steps;
+  for (int i = 0; i < 8 && e0 + i < total; ++i) {
+    const float v = (float)x.p[u * x.ss + t * x.rs + c] * d.scale;
+    y.p[u * y.ss + t * y.rs + c] = gone >> i & 1 ? (T)0.0f : (T)v;
+    if (++c == b.ncol) {
+      c = 0;
+      if (++t == b.steps) t = 0, ++u;   // packed rows: steps is 0, t never
+    }
+  }
+}
+
+// per = frame or sequence: a thread takes V columns of the 8 rows of one group of row numbers; its block decides the 8 rows, or
+// its column for as long as the sequence lasts.
+template <typename T, int V, bool FRAME>
+__global__ void __launch_bounds__(256) dropout_rows_kernel(const Batch b, const Split w, int64_t n_rows, const Dropout d,
+                                                           const Rows<const T> x, const Rows<T> y) {
+  const int slot = threadIdx.x / w.cb, group = blockIdx.y * w.cb + (threadIdx.x - slot * w.cb);
+  const int64_t r0 = ((int64_t)blockIdx.x * w.per + slot) * 8;
+  if (slot >= w.per || group >= w.groups || r0 >= n_rows) return;
+  const int col = group * V, k = (int)min((int64_t)8, n_rows - r0);
+  int64_t u = 0, end = n_rows;   // the sequence of a row, the first row behind it
+  if (b.steps) {
+    u = r0 / b.steps;
+    end = (u + 1) * b.steps;
+  } else if (!FRAME && b.off) {   // the last u with off[u] <= r0
+    int64_t hi = b.n_seq;
+    while (hi - u > 1) {
+      const int64_t mid = (u + hi) / 2;
+      if (b.off[mid] <= r0) u = mid; else hi = mid;
+    }
+    end = b.off[u + 1];
+  }
+  const int64_t step = d.at();
+  const int wide = (b.ncol + 7) / 8;
+  auto columns = [&]() { return philox_dropped((uint64_t)u * wide + col / 8, step, d.seed, d.threshold) >> (col & 7); };
+  uint32_t gone = FRAME ? philox_dropped((uint64_t)(r0 >> 3), step, d.seed, d.threshold) : columns();
+  const bool split = b.steps || (!FRAME && b.off);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (i >= k) break;
+    const int64_t r = r0 + i;
+    if (split && r >= end) {
+      do end = b.steps ? end + b.steps : b.off[++u + 1]; while (r >= end);
+      if (b.steps) u = end / b.steps - 1;
+      if (!FRAME) gone = columns();
+    }
+    const int64_t t = b.steps ? r - u * b.steps : r;
+    Pack<T, V> v;
+    load_pack<true>(v, x.p + (b.steps ? u * x.ss : 0) + t * x.rs + col);
+    float f[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = gone >> (FRAME ? i : j) & 1 ? 0.0f : (float)v.v[j] * d.scale;
+    store_pack<true, V>(y.p + (b.steps ? u * y.ss : 0) + t * y.rs + col, f);
+  }
 }
 
 }  // namespace mfcc

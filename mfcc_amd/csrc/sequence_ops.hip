@@ -1,5 +1,6 @@
 // C entry points of the operators along time (see "operators along time over feature rows" in include/mfcc_amd.h).
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "abi.h"
@@ -264,19 +265,41 @@ int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_ste
   if (const int rc = check_rows(who, "x", x, s, false)) return rc;
   if (const int rc = check_rows(who, "y", y, s, true)) return rc;
   if (state_in && state_in == state_out) return fail(MFCC_ERR_INVALID, "%s: state_out needs an array of its own", who);
-  const int64_t total = s.b.n_seq * ncol;
-  if (total == 0) return MFCC_OK;
-  auto go = [&](auto zero) {
-    using T = decltype(zero);
-    hipLaunchKernelGGL(mfcc::running_norm_kernel<T>, dim3(blocks_for(total, 256)), dim3(256), 0, (hipStream_t)stream, s.b,
-                       rows_of<const float>(x, s), rows_of<T>(y, s), decay, (float)eps, center_only ? 1 : 0, state_in, state_out);
+  if (y_dtype < 0 || y_dtype > MFCC_ROWS_F16) return bad_dtype(who, y_dtype);
+  if (s.b.n_seq == 0) return MFCC_OK;
+  Grid c = grid_of(s);
+  if (const int rc = check_grid(who, s, c, workspace)) return rc;
+  const size_t size = y_dtype == MFCC_ROWS_F32 ? 4 : 2;
+  const bool al = aligned(x, s, c.v, 4) && aligned(y, s, c.v, size);
+  c.w.near = near(x, c, s, 4) && near(y, c, s, size);
+  mfcc::NormArgs a;
+  a.decay = decay;
+  a.log_decay = std::log1p(decay - 1.0);
+  auto weights = [&](double k, double* decayed, double* grown) {
+    const double em = std::expm1(k * a.log_decay);
+    *decayed = 1.0 + em;
+    *grown = decay == 1.0 ? k : em / (decay - 1.0);
   };
-  switch (y_dtype) {
-    case MFCC_ROWS_F32: go(0.0f); break;
-    case MFCC_ROWS_BF16: go((mfcc::bf16)0.0f); break;
-    case MFCC_ROWS_F16: go((mfcc::f16)0.0f); break;
-    default: return bad_dtype(who, y_dtype);
+  weights(mfcc::kSlotRows, &a.slot_decay, &a.slot_grown);
+  weights(c.tile_rows, &a.tile_decay, &a.tile_grown);
+  for (int r = 0; r < mfcc::kSlotRows; ++r) {
+    double l, g;
+    weights(r + 1, &l, &g);
+    a.inv_grown[r] = (float)(1.0 / g);
   }
+  a.eps = (float)eps;
+  a.center_only = center_only ? 1 : 0;
+  a.state_in = state_in;
+  a.state_out = state_out;
+  a.runs = (float2*)workspace;
+  dispatch(y_dtype, c.v, al, [&](auto zero, auto v, auto al) {
+    using T = decltype(zero);
+    if (c.w.pieces > 1)
+      hipLaunchKernelGGL((mfcc::running_norm_pieces_kernel<v(), al()>), c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w,
+                         rows_of<const float>(x, s), a);
+    hipLaunchKernelGGL((mfcc::running_norm_kernel<T, v(), al()>), c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w,
+                       rows_of<const float>(x, s), rows_of<T>(y, s), a);
+  });
   HIP_TRY(hipGetLastError());
   return MFCC_OK;
 }
@@ -292,19 +315,38 @@ int mfcc_feature_dropout(const mfcc_layout* layout, int64_t n_seq, int64_t time_
   if (const int rc = check_rows(who, "x", x, s, false)) return rc;
   if (const int rc = check_rows(who, "y", y, s, true)) return rc;
   if (s.rows == 0) return MFCC_OK;
-  const float scale = threshold < 65536 ? 65536.0f / (float)(65536 - threshold) : 0.0f;
-  const int64_t total = s.rows * ncol;
-  if ((total + 255) / 256 > INT32_MAX) return fail(MFCC_ERR_UNSUPPORTED, "%s: too many rows per call", who);
-  auto go = [&](auto zero) {
-    using T = decltype(zero);
-    hipLaunchKernelGGL(mfcc::feature_dropout_kernel<T>, dim3(blocks_for(total, 256)), dim3(256), 0, (hipStream_t)stream, s.b, s.rows, per,
-                       (uint32_t)threshold, scale, seed, step, step_device, rows_of<const T>(x, s), rows_of<T>(y, s));
+  if (rows_dtype < 0 || rows_dtype > MFCC_ROWS_F16) return bad_dtype(who, rows_dtype);
+  const mfcc::Dropout d{seed, step, step_device, (uint32_t)threshold, threshold < 65536 ? 65536.0f / (float)(65536 - threshold) : 0.0f};
+  const size_t size = rows_dtype == MFCC_ROWS_F32 ? 4 : 2;
+  const int64_t most = (int64_t)INT32_MAX * 8;
+  hipStream_t st = (hipStream_t)stream;
+  // a batch without padding between its rows is one run of rows
+  auto flat = [&](const mfcc_rows* r) {
+    return r->row_stride == ncol && (s.b.steps == 0 || s.b.n_seq == 1 || r->seq_stride == s.b.steps * ncol) && (uintptr_t)r->data % 16 == 0;
   };
-  switch (rows_dtype) {
-    case MFCC_ROWS_F32: go(0.0f); break;
-    case MFCC_ROWS_BF16: go((mfcc::bf16)0.0f); break;
-    case MFCC_ROWS_F16: go((mfcc::f16)0.0f); break;
-    default: return bad_dtype(who, rows_dtype);
+  if (per == MFCC_DROP_ELEMENT) {
+    const int64_t blocks = (s.rows * ncol + 8 * 256 - 1) / (8 * 256);
+    if (blocks > INT32_MAX) return fail(MFCC_ERR_UNSUPPORTED, "%s: too many rows per call", who);
+    const bool fl = flat(x) && flat(y);
+    dispatch(rows_dtype, 1, true, [&](auto zero, auto, auto) {
+      using T = decltype(zero);
+      auto k = fl ? mfcc::dropout_element_kernel<T, true> : mfcc::dropout_element_kernel<T, false>;
+      hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(256), 0, st, s.b, s.rows, d, rows_of<const T>(x, s), rows_of<T>(y, s));
+    });
+  } else {
+    const int v = ncol % 2 == 0 && aligned(x, s, 2, size) && aligned(y, s, 2, size) ? 2 : 1;
+    mfcc::Split w{};
+    w.groups = ncol / v;
+    w.column_blocks = (w.groups + 255) / 256;
+    w.cb = (w.groups + w.column_blocks - 1) / w.column_blocks;
+    w.per = 256 / w.cb;
+    if (s.rows > most || w.column_blocks > 65535) return fail(MFCC_ERR_UNSUPPORTED, "%s: too many rows or columns per call", who);
+    const dim3 grid(blocks_for((s.rows + 7) / 8, w.per), (unsigned)w.column_blocks);
+    dispatch(rows_dtype, v, true, [&](auto zero, auto vv, auto) {
+      using T = decltype(zero);
+      auto k = per == MFCC_DROP_FRAME ? mfcc::dropout_rows_kernel<T, vv(), true> : mfcc::dropout_rows_kernel<T, vv(), false>;
+      hipLaunchKernelGGL(k, grid, dim3(256), 0, st, s.b, w, s.rows, d, rows_of<const T>(x, s), rows_of<T>(y, s));
+    });
   }
   HIP_TRY(hipGetLastError());
   return MFCC_OK;
