@@ -168,12 +168,21 @@ __device__ inline Lane<T> lane_of(const Rows<T>& r, const Batch& b, const Split&
   f.off = ((b.reverse ? w.per - 1 - t.sub : t.sub) * kSlotRows * (uint32_t)r.rs + t.col) * (uint32_t)sizeof(T);
   return f;
 }
+// The thread's offset, opaque, so that its extension to 64 bits stays next to the access: scalar base + 32-bit vector offset is
+// one addressing mode, and out of a loop the compiler would add them with vector instructions instead.
+__device__ inline uint32_t here(uint32_t off) {
+#ifdef __HIP__
+  asm("" : "+v"(off));
+#endif
+  return off;
+}
 template <bool FULL, bool AL, typename T, typename S, int V>
 __device__ inline void load_rows(Pack<T, V> (&r)[kSlotRows], const Lane<S>& f, const Seat& t, const Split& w, int tile) {
   if constexpr (FULL) {
     const char* p = f.base + tile * f.tile_step;
+    const uint32_t off = here(f.off);
 #pragma unroll
-    for (int i = 0; i < kSlotRows; ++i, p += f.row_step) load_pack<AL>(r[i], (const T*)(p + f.off));
+    for (int i = 0; i < kSlotRows; ++i, p += f.row_step) load_pack<AL>(r[i], (const T*)(p + off));
   } else {
     const int t0 = (tile * w.per + t.sub) * kSlotRows, last = max(t.n - 1, 0);
     const T* p = f.p + min(t0, last) * f.rs;
@@ -184,10 +193,10 @@ __device__ inline void load_rows(Pack<T, V> (&r)[kSlotRows], const Lane<S>& f, c
     }
   }
 }
-// Where row r of the thread's slot goes.
+// Where row r of the thread's slot goes (off: its offset, here()).
 template <bool FULL, typename T>
-__device__ inline T* row_at(const Lane<T>& f, const Seat& t, const Split& w, int tile, int r) {
-  if constexpr (FULL) return (T*)(f.base + tile * f.tile_step + r * f.row_step + f.off);
+__device__ inline T* row_at(const Lane<T>& f, const Seat& t, const Split& w, int tile, int r, uint32_t off) {
+  if constexpr (FULL) return (T*)(f.base + tile * f.tile_step + r * f.row_step + off);
   return (T*)f.p + ((tile * w.per + t.sub) * kSlotRows + r) * f.rs;
 }
 
@@ -195,6 +204,38 @@ template <bool AL, int V, typename T>
 __device__ inline void zero_behind(const Rows<T>& y, const Batch& b, const Split& w, const Seat& t) {
   const float z[V] = {};
   for (int64_t r = t.n + t.piece * w.per + t.sub; r < b.steps; r += w.pieces * w.per) store_pack<AL, V>(y.p + t.u * y.ss + r * y.rs + t.col, z);
+}
+
+// The rows of a slot's run of a piece: `run` neighbouring rows from row `begin` on, R at a time.
+template <typename T>
+struct RunLane {
+  Lane<T> f;
+  const char* base;
+  uint32_t off;
+};
+template <typename T>
+__device__ inline RunLane<T> run_of(const Lane<T>& f, const Rows<T>& r, const Batch& b, const Split& w, const Seat& t, int run) {
+  RunLane<T> l{f, nullptr, 0};
+  const int64_t back = b.reverse ? (int64_t)(w.per - 1) * r.rs * sizeof(T) : 0;   // the last slot is the lowest one in reverse
+  l.base = f.base + t.tile * f.tile_step + kSlotRows * back - run * back;
+  l.off = ((b.reverse ? w.per - 1 - t.sub : t.sub) * run * (uint32_t)r.rs + t.col) * (uint32_t)sizeof(T);
+  return l;
+}
+template <bool FULL, bool AL, typename T, typename S, int V>
+__device__ inline void load_run(Pack<T, V> (&r)[kSlotRows], const RunLane<S>& l, const Seat& t, int begin, int at) {
+  if constexpr (FULL) {
+    const char* p = l.base + at * l.f.row_step;
+    const uint32_t off = here(l.off);
+#pragma unroll
+    for (int i = 0; i < kSlotRows; ++i, p += l.f.row_step) load_pack<AL>(r[i], (const T*)(p + off));
+  } else {
+    const T* p = l.f.p + min(begin + at, t.n - 1) * l.f.rs;
+#pragma unroll
+    for (int i = 0; i < kSlotRows; ++i) {
+      load_pack<AL>(r[i], p);
+      p += begin + at + i < t.n - 1 ? l.f.rs : 0;
+    }
+  }
 }
 
 // ---- gated recurrence -----------------------------------------------------------------------------
@@ -237,41 +278,41 @@ __global__ void __launch_bounds__(kSeqThreads, 4) gated_scan_pieces_kernel(const
   const Seat t = seat_of<V>(b, w);
   if (!t.there || t.tile >= t.tiles || !g.p) return;   // the same for the whole workgroup
   const bool no_gy = BACK && !x.p;
-  const Lane<const T> fg = lane_of<V>(g, b, w, t), fx = no_gy ? fg : lane_of<V>(x, b, w, t);
+  const int run = w.piece_tiles * R, piece = t.tile * w.per * R, first = piece + t.sub * run;
+  const RunLane<const T> fg = run_of(lane_of<V>(g, b, w, t), g, b, w, t, run);
+  const RunLane<const T> fx = no_gy ? fg : run_of(lane_of<V>(x, b, w, t), x, b, w, t, run);
   float A[V], X[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) A[v] = 1.0f, X[v] = 0.0f;
-  const int run = w.piece_tiles * R, first = t.tile * w.per * R + t.sub * run;
-  const int len = min(max(t.n - first, 0), run), last = BACK ? (len + R - 1) / R * R - R : 0;
-  auto load = [&](ScanRows<T, V>& r, int at) {
-    const T *px = fx.p + min(first + at, t.n - 1) * fx.rs, *pg = fg.p + min(first + at, t.n - 1) * fg.rs;
+  auto walk = [&](auto full) {
+    constexpr bool FULL = full();
+    const int len = FULL ? run : min(max(t.n - first, 0), run), last = BACK ? (len + R - 1) / R * R - R : 0;
+    auto load = [&](ScanRows<T, V>& r, int at) {
+      load_run<FULL, AL>(r.x, fx, t, first, at);
+      load_run<FULL, AL>(r.g, fg, t, first, at);
+    };
+    ScanRows<T, V> in, next;
+    load(in, last);
+    for (int i = 0; i < len; i += R) {
+      const int at = BACK ? last - i : i, k = len - at;
+      load(next, BACK ? max(at - R, 0) : FULL ? min(at + R, run - R) : at + R);
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      load_pack<AL>(r.x[i], px);
-      load_pack<AL>(r.g[i], pg);
-      px += first + at + i < t.n - 1 ? fx.rs : 0;
-      pg += first + at + i < t.n - 1 ? fg.rs : 0;
+      for (int j = 0; j < R; ++j)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int r = BACK ? R - 1 - j : j;
+          float a = (float)in.g[r].v[v], na = 1.0f;
+          if constexpr (SIG) sigmoid2(a, a, na);
+          const float xv = no_gy ? 0.0f : (float)in.x[r].v[v];
+          const float nx = BACK ? a * (xv + X[v]) : fmaf(a, X[v], na * xv);
+          X[v] = FULL || r < k ? nx : X[v];
+          A[v] = FULL || r < k ? A[v] * a : A[v];
+        }
+      in = next;
     }
   };
-  ScanRows<T, V> in, next;
-  load(in, last);
-  for (int i = 0; i < len; i += R) {
-    const int at = BACK ? last - i : i, k = len - at;
-    load(next, BACK ? max(at - R, 0) : at + R);
-#pragma unroll
-    for (int j = 0; j < R; ++j)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const int r = BACK ? R - 1 - j : j;
-        float a = (float)in.g[r].v[v], na = 1.0f;
-        if constexpr (SIG) sigmoid2(a, a, na);
-        const float xv = no_gy ? 0.0f : (float)in.x[r].v[v];
-        const float nx = BACK ? a * (xv + X[v]) : fmaf(a, X[v], na * xv);
-        X[v] = r < k ? nx : X[v];
-        A[v] = r < k ? A[v] * a : A[v];
-      }
-    in = next;
-  }
+  if (w.near && piece + w.per * run <= t.n) walk(std::true_type());
+  else walk(std::false_type());
 #pragma unroll
   for (int v = 0; v < V; ++v) maps[(t.slot * V + v) * w.cb + t.cg] = make_float2(A[v], X[v]);
   __syncthreads();
@@ -374,11 +415,12 @@ __global__ void __launch_bounds__(kSeqThreads, 4) gated_scan_kernel(const Batch 
     if (ck && t.sub == 0 && k > 0)
 #pragma unroll
       for (int v = 0; v < V; ++v) ck[(int64_t)tile * b.ncol + v] = h[v];
+    const uint32_t to = here(fy.off);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
 #pragma unroll
       for (int v = 0; v < V; ++v) h[v] = fmaf(a[r][v], h[v], x1[r][v]);
-      if (FULL || r < k) store_pack<AL, V>(row_at<FULL>(fy, t, w, tile, r), h);
+      if (FULL || r < k) store_pack<AL, V>(row_at<FULL>(fy, t, w, tile, r, to), h);
     }
   };
 
@@ -502,6 +544,7 @@ __global__ void __launch_bounds__(kSeqThreads, 2) gated_scan_backward_kernel(con
           hp[r][v] = h[v];
           h[v] = fmaf(a[r][v], h[v], FULL || r < k ? na[r][v] * (float)in.x[r].v[v] : 0.0f);
         }
+      const uint32_t to_x = here(fgx.off), to_g = here(fgg.off);
 #pragma unroll
       for (int r = R - 1; r >= 0; --r) {
         float dx[V], dg[V];
@@ -513,8 +556,8 @@ __global__ void __launch_bounds__(kSeqThreads, 2) gated_scan_backward_kernel(con
           dg[v] = SIG ? e[v] * na[r][v] * (hp[r][v] - (float)in.x[r].v[v]) : d * hp[r][v];
         }
         if (FULL || r < k) {
-          store_pack<AL, V>(row_at<FULL>(fgx, t, w, tile, r), dx);
-          store_pack<AL, V>(row_at<FULL>(fgg, t, w, tile, r), dg);
+          store_pack<AL, V>(row_at<FULL>(fgx, t, w, tile, r, to_x), dx);
+          store_pack<AL, V>(row_at<FULL>(fgg, t, w, tile, r, to_g), dg);
         }
       }
     }
@@ -576,11 +619,12 @@ __global__ void __launch_bounds__(256) gated_scan_step_kernel(int64_t n, int nco
 // point of w the roundings of 32 bits have one sign: 7e-6 of w off after 20000 rows at decay 0.995), and f and decay^k w f are
 // computed once per slot. The mean that enters a tile is carried in 64 bits and the tile composes 32-bit deviations from it: a
 // cumulative mean of n rows would otherwise collect sqrt(n) / 4 units in the last place.
-// Bound: HBM, one value read and one written; 25 operations a value.
+// Bound: HBM, one value read and one written; about 35 instructions a value, so slots are few where sequences are many (every
+// join is shared by R values only).
 struct NormArgs {
   double decay, log_decay;      // log_decay = log1p(decay - 1)
   double slot_decay, slot_grown, tile_decay, tile_grown;   // decay^k and g(k) of a slot and of a tile
-  float eps, inv_grown[kSlotRows];   // 1 / g(1) .. 1 / g(R)
+  float eps, decayed[kSlotRows], grown[kSlotRows], inv_grown[kSlotRows];   // decay^k, g(k), 1 / g(k) for k = 1 .. R
   int center_only;
   const float* state_in;
   float* state_out;
@@ -624,25 +668,24 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_pieces_kernel(con
   __shared__ float2 runs[kSeqThreads * V];
   const Seat t = seat_of<V>(b, w);
   if (!t.there || t.tile >= t.tiles || !x.p) return;   // the same for the whole workgroup
-  const Lane<const float> fx = lane_of<V>(x, b, w, t);
-  const int run = w.piece_tiles * R, first = t.tile * w.per * R, begin = first + t.sub * run, len = min(max(t.n - begin, 0), run);
-  auto load = [&](Pack<float, V>(&r)[R], int at) {
-    const float* p = fx.p + min(begin + at, t.n - 1) * fx.rs;
+  const int run = w.piece_tiles * R, first = t.tile * w.per * R, begin = first + t.sub * run;
+  const RunLane<const float> fx = run_of(lane_of<V>(x, b, w, t), x, b, w, t, run);
+  float m[V] = {}, q[V] = {};
+  auto walk = [&](auto full) {
+    constexpr bool FULL = full();
+    const int len = FULL ? run : min(max(t.n - begin, 0), run);
+    float sum = 0.0f;
+    Pack<float, V> in[R], next[R];
+    load_run<FULL, AL>(in, fx, t, begin, 0);
+    for (int i = 0; i < len; i += R) {
+      load_run<FULL, AL>(next, fx, t, begin, FULL ? min(i + R, run - R) : i + R);
+      norm_run<V, R, FULL>(m, q, sum, (float)a.decay, in, len - i, nullptr);
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      load_pack<AL>(r[i], p);
-      p += begin + at + i < t.n - 1 ? fx.rs : 0;
+      for (int r = 0; r < R; ++r) in[r] = next[r];
     }
   };
-  Pack<float, V> in[R], next[R];
-  float m[V] = {}, q[V] = {}, sum = 0.0f;
-  load(in, 0);
-  for (int i = 0; i < len; i += R) {
-    load(next, i + R);
-    norm_run<V, R, false>(m, q, sum, (float)a.decay, in, len - i, nullptr);
-#pragma unroll
-    for (int r = 0; r < R; ++r) in[r] = next[r];
-  }
+  if (w.near && first + w.per * run <= t.n) walk(std::true_type());
+  else walk(std::false_type());
 #pragma unroll
   for (int v = 0; v < V; ++v) runs[(t.slot * V + v) * w.cb + t.cg] = make_float2(m[v], q[v]);
   __syncthreads();
@@ -672,10 +715,15 @@ template <typename T, int V, bool AL>
 __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batch b, const Split w, const Rows<const float> x, const Rows<T> y,
                                                                       const NormArgs a) {
   constexpr int R = kSlotRows;
-  __shared__ float2 runs[2][kSeqThreads * V];
-  __shared__ float4 joins[2][kSeqThreads];   // of every slot: f, decay^k w f, decay^k
+  // twice, for tiles in turn: the run of every (slot, column); of every slot the weights of its join, (f, decay^k w f, decay^k, -), and
+  // 1 / w of its rows
+  extern __shared__ float4 shared[];
   const Seat t = seat_of<V>(b, w);
   if (!t.there) return;
+  const int slots = w.seqs * w.per;
+  float4* const joins = shared;
+  float4* const inverses = joins + 2 * slots;
+  float2* const runs = (float2*)(inverses + 2 * slots * (R / 4));
   const Lane<const float> fx = lane_of<V>(x, b, w, t);
   const Lane<T> fy = lane_of<V>(y, b, w, t);
   const float decay = (float)a.decay;
@@ -683,8 +731,9 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batc
   // decay^k and g(k) of the rows of a tile before the thread's slot
   double before_decay = 1.0, before_grown = 0.0;
   for (int s = 0; s < t.sub; ++s) before_decay *= a.slot_decay, before_grown = fma(a.slot_decay, before_grown, a.slot_grown);
+  const float own_decayed = a.decayed[min(t.cg, R - 1)], own_grown = a.grown[min(t.cg, R - 1)];   // read here: a load in the loop waits for all others
   double weight = 0.0, mean[V] = {};   // that enter the tile
-  float square[V] = {}, m[V] = {}, q[V] = {};
+  float square[V] = {}, m[V] = {}, q[V] = {}, last_weight = 0.0f;
   if (t.on && a.state_in) {
     weight = a.state_in[state];
 #pragma unroll
@@ -693,66 +742,77 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batc
 
   auto work = [&](auto full, const Pack<float, V>(&in)[R], int tile) {
     constexpr bool FULL = full();
-    const int k = FULL ? R : min(max(t.n - (tile * w.per + t.sub) * R, 0), R);
-    float ws = (float)fma(before_decay, weight, before_grown);
+    const int k = FULL ? R : min(max(t.n - (tile * w.per + t.sub) * R, 0), R), turn = tile & 1;
+    const float ws = (float)fma(before_decay, weight, before_grown);
+    last_weight = fmaf(FULL || k == R ? a.decayed[R - 1] : k > 0 ? a.decayed[k - 1] : 1.0f, ws, FULL || k == R ? a.grown[R - 1] : k > 0 ? a.grown[k - 1] : 0.0f);
     float base[V], off[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) base[v] = (float)mean[v], off[v] = (float)(mean[v] - base[v]);
+    float4* const inv = inverses + (turn * slots + t.slot) * (R / 4);
+    // 1 / w of the rows: the first column groups take one row each
+    if (t.cg < R) ((float*)inv)[t.cg] = __builtin_amdgcn_rcpf(fmaf(own_decayed, ws, own_grown));
+    for (int r = t.cg + w.cb; r < R; r += w.cb) ((float*)inv)[r] = __builtin_amdgcn_rcpf(fmaf(a.decayed[r], ws, a.grown[r]));   // few columns
     if (w.per > 1) {
 #pragma unroll
       for (int v = 0; v < V; ++v) m[v] = 0.0f, q[v] = 0.0f;
       float none = 0.0f;
       norm_run<V, R, FULL>(m, q, none, decay, in, k, a.inv_grown);
-      float l = (float)a.slot_decay, g = (float)a.slot_grown;
-      if (!FULL && k < R) {
-        l = 1.0f, g = 0.0f;
-        for (int r = 0; r < k; ++r) l *= decay, g = fmaf(decay, g, 1.0f);
-      }
-      const float old = l * ws, f = g == 0.0f ? 0.0f : old > 0.0f ? g * __builtin_amdgcn_rcpf(old + g) : 1.0f;   // a first run is its own mean
-      float2* const e = runs[tile & 1];
-      float4* const j = joins[tile & 1];
+      float4* const j = joins + turn * slots;
+      float2* const e = runs + turn * slots * V * w.cb + t.cg;
 #pragma unroll
-      for (int v = 0; v < V; ++v) e[(t.slot * V + v) * w.cb + t.cg] = make_float2(m[v], q[v]);
-      if (t.cg == 0) j[t.slot] = make_float4(f, old * f, l, 0.0f);
+      for (int v = 0; v < V; ++v) e[(t.slot * V + v) * w.cb] = make_float2(m[v] - base[v], q[v]);
+      if (t.cg == 0) {
+        const float l = FULL || k == R ? a.decayed[R - 1] : k > 0 ? a.decayed[k - 1] : 1.0f;
+        const float g = FULL || k == R ? a.grown[R - 1] : k > 0 ? a.grown[k - 1] : 0.0f;
+        const float old = l * ws, f = g == 0.0f ? 0.0f : old > 0.0f ? g * __builtin_amdgcn_rcpf(old + g) : 1.0f;   // a first run is its own mean
+        j[t.slot] = make_float4(f, old * f, l, 0.0f);
+      }
       __syncthreads();
-      const int first = t.slot - t.sub;
-#pragma unroll 2
-      for (int s = 0; s < w.per; ++s) {
-        const float4 p = j[first + s];
+      const float2* r = e + (t.slot - t.sub) * V * w.cb;
+      const float4* p = j + (t.slot - t.sub);
+      auto join = [&]() {
+        const float4 h = *p++;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float2 r = e[((first + s) * V + v) * w.cb + t.cg];
-          m[v] = s == t.sub ? off[v] : m[v];
-          q[v] = s == t.sub ? square[v] : q[v];
-          const float d = r.x - base[v] - off[v];
-          off[v] = fmaf(d, p.x, off[v]);
-          square[v] = fmaf(p.z, square[v], fmaf(d * d, p.y, r.y));
+        for (int v = 0; v < V; ++v, r += w.cb) {
+          const float2 run = *r;
+          const float d = run.x - off[v];
+          off[v] = fmaf(d, h.x, off[v]);
+          square[v] = fmaf(h.z, square[v], fmaf(d * d, h.y, run.y));
         }
-      }
+      };
+      int i = 0;
+#pragma unroll 4
+      for (; i < t.sub; ++i) join();
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        mean[v] = (double)base[v] + off[v];
-        m[v] += base[v];
-      }
+      for (int v = 0; v < V; ++v) m[v] = base[v] + off[v], q[v] = square[v];
+#pragma unroll 4
+      for (; i < w.per; ++i) join();
+#pragma unroll
+      for (int v = 0; v < V; ++v) mean[v] = (double)base[v] + off[v];
       weight = fma(a.tile_decay, weight, a.tile_grown);   // behind a last tile with missing rows it is not used
     } else {
-      __syncthreads();   // doubles have read their rows: y may be x
+      __syncthreads();   // 1 / w; and doubles have read their rows: y may be x
 #pragma unroll
       for (int v = 0; v < V; ++v) m[v] = base[v], q[v] = square[v];
     }
+    const uint32_t to = here(fy.off);
+    float f[R];
+#pragma unroll
+    for (int r = 0; r < R; r += 4) {
+      const float4 four = inv[r / 4];
+      f[r] = four.x, f[r + 1] = four.y, f[r + 2] = four.z, f[r + 3] = four.w;
+    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      ws = fmaf(decay, ws, 1.0f);
-      const float f = __builtin_amdgcn_rcpf(ws);
       float o[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float d = in[r].v[v] - m[v], mn = fmaf(d, f, m[v]), c = in[r].v[v] - mn, qn = fmaf(d, c, decay * q[v]);
-        o[v] = a.center_only ? c : c * __builtin_amdgcn_rsqf(fmaf(qn, f, a.eps));
+        const float d = in[r].v[v] - m[v], mn = fmaf(d, f[r], m[v]), c = in[r].v[v] - mn, qn = fmaf(d, c, decay * q[v]);
+        o[v] = a.center_only ? c : c * __builtin_amdgcn_rsqf(fmaf(qn, f[r], a.eps));
         m[v] = FULL || r < k ? mn : m[v];
         q[v] = FULL || r < k ? qn : q[v];
       }
-      if (FULL || r < k) store_pack<AL, V>(row_at<FULL>(fy, t, w, tile, r), o);
+      if (FULL || r < k) store_pack<AL, V>(row_at<FULL>(fy, t, w, tile, r, to), o);
     }
   };
 
@@ -778,7 +838,7 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batc
         sum = wn;
       }
 #pragma unroll
-      for (int v = 0; v < V; ++v) runs[0][(t.slot * V + v) * w.cb + t.cg] = make_float2(m[v], q[v]);
+      for (int v = 0; v < V; ++v) runs[(t.slot * V + v) * w.cb + t.cg] = make_float2(m[v], q[v]);
       __syncthreads();
       weights_of(a, (double)run * w.piece_tiles * w.per * R, lr, gr);
       for (int s = 0; s < w.per && s * run < t.piece; ++s) {
@@ -786,7 +846,7 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batc
         const double old = lr * weight, f = gr / (old + gr);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float2 e = runs[0][(s * V + v) * w.cb + t.cg];
+          const float2 e = runs[(s * V + v) * w.cb + t.cg];
           const double d = e.x - mean[v];
           mean[v] = fma(d, f, mean[v]);
           square[v] = (float)(lr * square[v] + e.y + d * d * old * f);
@@ -815,13 +875,12 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batc
   // the state behind the last row, from the thread that walked it
   const int lead = t.n > 0 ? (t.n - 1) / R % w.per : 0;
   if (t.on && a.state_out && t.sub == lead && (t.n > 0 ? t.tile < t.tiles && t.tiles * w.per * R >= t.n : t.piece == 0)) {
-    double l, g;
-    weights_of(a, t.n, l, g);
-    if (t.col == 0) a.state_out[state] = (float)(l * (a.state_in ? (double)a.state_in[state] : 0.0) + g);
+    auto entered = [&](int64_t i) { return a.state_in ? a.state_in[state + i] : 0.0f; };   // passes through where there are no rows
+    if (t.col == 0) a.state_out[state] = t.n > 0 ? last_weight : entered(0);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      a.state_out[state + 1 + t.col + v] = t.n > 0 ? m[v] : (float)mean[v];
-      a.state_out[state + 1 + b.ncol + t.col + v] = t.n > 0 ? q[v] : square[v];
+      a.state_out[state + 1 + t.col + v] = t.n > 0 ? m[v] : entered(1 + t.col + v);
+      a.state_out[state + 1 + b.ncol + t.col + v] = t.n > 0 ? q[v] : entered(1 + b.ncol + t.col + v);
     }
   }
   if (t.on && b.steps) zero_behind<AL, V>(y, b, w, t);

@@ -55,6 +55,9 @@ int check_rows(const char* who, const char* name, const mfcc_rows* r, const Shap
 // 17.1 (38.8).  32 sequences of up to 700 rows (11 tiles, 4 pieces would fill the card) 18.9 us whole, 28 in pieces.
 constexpr int64_t kFewBlocks = 256, kManyTiles = 10, kManyPieces = 5, kTargetBlocks = 512, kPieceTiles = 2;
 
+// Workgroups of half the threads for the normalisation where there are many: half the slots to join a tile.
+constexpr int64_t kManyBlocks = 2048;
+
 // How workgroups divide sequences, columns and time.  It depends on the shape of the batch alone, so that the backward
 // pass finds its checkpoints whatever the alignment of its arrays.
 struct Grid {
@@ -62,7 +65,7 @@ struct Grid {
   mfcc::Split w;
   dim3 blocks;
 };
-Grid grid_of(const Shape& s) {
+Grid grid_of(const Shape& s, int threads = mfcc::kSeqThreads) {
   Grid g;
   g.v = s.b.ncol % 2 ? 1 : 2;   // values of a row that a thread takes at once
   g.w.groups = s.b.ncol / g.v;
@@ -73,7 +76,7 @@ Grid grid_of(const Shape& s) {
   auto split = [&](int wide) {
     g.w.column_blocks = (g.w.groups + wide - 1) / wide;
     g.w.cb = (g.w.groups + g.w.column_blocks - 1) / g.w.column_blocks;
-    const int slots = mfcc::kSeqThreads / g.w.cb;
+    const int slots = threads / g.w.cb;
     const int64_t need = std::max<int64_t>(1, (s.longest + mfcc::kSlotRows - 1) / mfcc::kSlotRows);
     g.w.per = (int32_t)std::min<int64_t>(std::min(slots, 64), need);
     g.w.seqs = need <= g.w.per ? slots / g.w.per : 1;
@@ -84,7 +87,7 @@ Grid grid_of(const Shape& s) {
   split(64);   // a wave to a row
   const int64_t blocks = (int64_t)g.w.blocks * g.w.column_blocks, tiles = g.w.piece_tiles;
   if (g.w.seqs == 1 && blocks > 0 && blocks < kFewBlocks) {
-    const int64_t want = std::min((kTargetBlocks + blocks - 1) / blocks, tiles / kPieceTiles);
+    const int64_t want = std::min(kTargetBlocks / blocks, tiles / kPieceTiles);   // not one more than the card takes at once
     if (tiles >= kManyTiles && want >= kManyPieces) {
       g.w.piece_tiles = (int32_t)((tiles + want - 1) / want);
       g.w.pieces = (int32_t)((tiles + g.w.piece_tiles - 1) / g.w.piece_tiles);
@@ -109,9 +112,10 @@ bool aligned(const mfcc_rows* r, const Shape& s, int v, size_t size) {
   return !r || (((uintptr_t)r->data % (v * size)) == 0 && r->row_stride % v == 0 && (s.b.steps == 0 || r->seq_stride % v == 0));
 }
 
-// Offsets inside a tile are 32-bit numbers of bytes where that is enough.
+// Offsets inside a tile (a piece) are 32-bit numbers of bytes where that is enough.
 bool near(const mfcc_rows* r, const Grid& c, const Shape& s, size_t size) {
-  return !r || (c.tile_rows * (double)r->row_stride + s.b.ncol) * size < 4294967296.0;
+  const double rows = (double)c.tile_rows * (c.w.pieces > 1 ? c.w.piece_tiles : 1);
+  return !r || (rows * (double)r->row_stride + s.b.ncol) * size < 4294967296.0;
 }
 
 // f(type's zero, number of values, aligned) for the row type, the values a thread takes and the alignment of the arrays
@@ -269,6 +273,8 @@ int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_ste
   if (s.b.n_seq == 0) return MFCC_OK;
   Grid c = grid_of(s);
   if (const int rc = check_grid(who, s, c, workspace)) return rc;
+  int threads = mfcc::kSeqThreads;
+  if (c.w.pieces == 1 && (int64_t)c.w.blocks * c.w.column_blocks >= kManyBlocks) c = grid_of(s, threads = mfcc::kSeqThreads / 2);
   const size_t size = y_dtype == MFCC_ROWS_F32 ? 4 : 2;
   const bool al = aligned(x, s, c.v, 4) && aligned(y, s, c.v, size);
   c.w.near = near(x, c, s, 4) && near(y, c, s, size);
@@ -285,6 +291,8 @@ int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_ste
   for (int r = 0; r < mfcc::kSlotRows; ++r) {
     double l, g;
     weights(r + 1, &l, &g);
+    a.decayed[r] = (float)l;
+    a.grown[r] = (float)g;
     a.inv_grown[r] = (float)(1.0 / g);
   }
   a.eps = (float)eps;
@@ -297,7 +305,9 @@ int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_ste
     if (c.w.pieces > 1)
       hipLaunchKernelGGL((mfcc::running_norm_pieces_kernel<v(), al()>), c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w,
                          rows_of<const float>(x, s), a);
-    hipLaunchKernelGGL((mfcc::running_norm_kernel<T, v(), al()>), c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w,
+    const int slots = c.w.seqs * c.w.per;
+    const size_t shared = 2 * slots * ((1 + mfcc::kSlotRows / 4) * sizeof(float4) + v() * c.w.cb * sizeof(float2));
+    hipLaunchKernelGGL((mfcc::running_norm_kernel<T, v(), al()>), c.blocks, dim3(threads), shared, (hipStream_t)stream, s.b, c.w,
                        rows_of<const float>(x, s), rows_of<T>(y, s), a);
   });
   HIP_TRY(hipGetLastError());

@@ -24,13 +24,13 @@ _FORMS = {"decay": capi.SCAN_DECAY, "sigmoid": capi.SCAN_SIGMOID}
 _PER = {"element": capi.DROP_ELEMENT, "frame": capi.DROP_FRAME, "sequence": capi.DROP_SEQUENCE}
 
 
-def _stream():
-    return torch.cuda.current_stream().cuda_stream
+# the handle of a device's current stream, without the Stream object that torch.cuda.current_stream() builds (3 us of a 13 us call)
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 class _Batch:
     """Geometry of one call: the layout handle, the number of sequences, the padded length (0 = packed)."""
-    __slots__ = ("layout", "handle", "n_seq", "steps", "ncol")
+    __slots__ = ("layout", "handle", "n_seq", "steps", "ncol", "device")
 
     def __init__(self, x, frame_counts):
         if x.dim() not in (2, 3):
@@ -39,6 +39,7 @@ class _Batch:
         if self.ncol < 1:
             raise ValueError("rows without columns")
         self.layout = None
+        self.device = x.device.index
         if frame_counts is not None:
             if not isinstance(frame_counts, Layout):
                 if torch.cuda.is_current_stream_capturing():
@@ -113,9 +114,21 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _workspace(batch, dtype, device):
-    n = capi.check(capi.load().mfcc_sequence_workspace(*batch.head(), _ROWS[dtype]))
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+def _sizes(batch, code):
+    """(checkpoint floats, workspace bytes) of a batch, asked for once per shape"""
+    known = _plain_sizes if batch.layout is None else batch.layout.__dict__.setdefault("_sequence_sizes", {})
+    key = (batch.n_seq, batch.steps, batch.ncol, code)
+    found = known.get(key)
+    if found is None:
+        lib = capi.load()
+        if len(known) > 256:
+            known.clear()
+        found = known[key] = (capi.check(lib.mfcc_gated_scan_checkpoints(*batch.head(), code)),
+                              capi.check(lib.mfcc_sequence_workspace(*batch.head(), code)))
+    return found
+
+
+_plain_sizes = {}
 
 
 def _no_grad(*tensors):
@@ -130,13 +143,12 @@ def _scan_forward(x, gate, h0, batch, form, reverse, out, keep):
     y = _out(out, x.shape, x.dtype, x.device)
     last = torch.empty((batch.n_seq, batch.ncol), dtype=torch.float32, device=x.device)
     code = _ROWS[x.dtype]
+    n_ckpt, n_ws = _sizes(batch, code)
     with _on(x.device, gate, h0, y):
-        ckpt = None
-        if keep:
-            ckpt = torch.empty(capi.check(lib.mfcc_gated_scan_checkpoints(*batch.head(), code)), dtype=torch.float32, device=x.device)
-        ws = _workspace(batch, x.dtype, x.device)
+        ckpt = torch.empty(n_ckpt, dtype=torch.float32, device=x.device) if keep else None
+        ws = torch.empty(n_ws, dtype=torch.uint8, device=x.device) if n_ws else None
         capi.check(lib.mfcc_gated_scan(*batch.head(), code, form, reverse, _rows(x), _rows(gate), _ptr(h0), _rows(y), last.data_ptr(),
-                                       _ptr(ckpt), _ptr(ws), _stream()))
+                                       _ptr(ckpt), _ptr(ws), _stream(batch.device)))
     return y, last, ckpt
 
 
@@ -163,10 +175,11 @@ class _GatedScan(torch.autograd.Function):
         gx, gg = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(x.shape, dtype=x.dtype, device=x.device)
         gh0 = torch.empty((batch.n_seq, batch.ncol), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
         with _on(x.device, gy, glast):
-            ws = _workspace(batch, x.dtype, x.device)
+            n_ws = _sizes(batch, _ROWS[x.dtype])[1]
+            ws = torch.empty(n_ws, dtype=torch.uint8, device=x.device) if n_ws else None
             capi.check(capi.load().mfcc_gated_scan_backward(
                 *batch.head(), _ROWS[x.dtype], form, reverse, _rows(x), _rows(gate), ckpt.data_ptr(), None if gy is None else _rows(gy),
-                _ptr(glast), _rows(gx), _rows(gg), _ptr(gh0), _ptr(ws), _stream()))
+                _ptr(glast), _rows(gx), _rows(gg), _ptr(gh0), _ptr(ws), _stream(batch.device)))
         need = ctx.needs_input_grad
         return gx if need[0] else None, gg if need[1] else None, gh0, None, None, None
 
@@ -223,7 +236,7 @@ def gated_scan_step(x, gate, state, form="decay", out=None, state_out=None):
     n, d = x.shape
     with _on(x.device, gate, state, state_out, y):
         capi.check(capi.load().mfcc_gated_scan_step(n, d, _ROWS[x.dtype], _FORMS[form], x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0),
-                                                    state.data_ptr(), state_out.data_ptr(), y.data_ptr(), y.stride(0), _stream()))
+                                                    state.data_ptr(), state_out.data_ptr(), y.data_ptr(), y.stride(0), _stream(x.device.index)))
     return y, state_out
 
 
@@ -264,9 +277,10 @@ def running_norm(feats, frame_counts=None, decay=0.995, state=None, eps=1e-5, ce
     if state is not None and not state.is_contiguous():
         state = state.contiguous()
     with _on(feats.device, state, state_out, y):
-        ws = _workspace(batch, torch.float32, feats.device)
+        n_ws = _sizes(batch, capi.ROWS_F32)[1]
+        ws = torch.empty(n_ws, dtype=torch.uint8, device=feats.device) if n_ws else None
         capi.check(capi.load().mfcc_running_norm(*batch.head(), decay, eps, int(bool(center_only)), _rows(feats), _ptr(state), _rows(y),
-                                                 _ROWS[dtype], state_out.data_ptr(), _ptr(ws), _stream()))
+                                                 _ROWS[dtype], state_out.data_ptr(), _ptr(ws), _stream(batch.device)))
     return y, state_out
 
 
@@ -292,7 +306,7 @@ def _drop(x, batch, per, threshold, seed, step, out):
     on_device = isinstance(step, torch.Tensor)
     with _on(x.device, y, step if on_device else None):
         capi.check(capi.load().mfcc_feature_dropout(*batch.head(), _ROWS[x.dtype], per, threshold, seed, 0 if on_device else step,
-                                                    step.data_ptr() if on_device else None, _rows(x), _rows(y), _stream()))
+                                                    step.data_ptr() if on_device else None, _rows(x), _rows(y), _stream(batch.device)))
     return y
 
 
