@@ -7,8 +7,9 @@ SEQ   := mfcc_amd/csrc/sequence_ops.hip
 SEQO  := build/sequence_ops.o
 HDRS  := $(wildcard mfcc_amd/csrc/*.h) include/mfcc_amd.h
 HIPFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -fno-signed-zeros -fno-slp-vectorize -Wall -Wno-unused-function
-# the operators along time: no packed float32 instructions (some of their forms have given wrong results on this part)
-SEQFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -c -fno-slp-vectorize -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops
+# the operators along time: no packed float32 instructions (some of their forms have given wrong results on this part), and no
+# contraction of products and sums by the compiler, so that full and partial tiles round alike (fused where the source says fmaf)
+SEQFLAGS := --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -c -fno-slp-vectorize -ffp-contract=off -Wall -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops
 
 all: $(LIB) host_sim
 

@@ -307,7 +307,7 @@ int mfcc_gated_scan(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps
                     int32_t reverse, const mfcc_rows* x, const mfcc_rows* gate, const float* h0, const mfcc_rows* y, float* last,
                     float* checkpoints, void* workspace, void* stream);
 /* Gradients of mfcc_gated_scan: from grad_y (rows; NULL = 0) and grad_last (float32 [n_seq, ncol]; NULL = 0) to grad_x,
- * grad_gate (rows) and grad_h0 (float32 [n_seq, ncol]; may be NULL).  x, gate, h0, checkpoints and the geometry are the
+ * grad_gate (rows) and grad_h0 (float32 [n_seq, ncol]; may be NULL), which overlap none of the inputs.  x, gate, h0, checkpoints and the geometry are the
  * forward call's.  The states are computed again in float32 from the checkpoints, so grad_gate does not suffer from
  * the rounding of y. */
 int mfcc_gated_scan_backward(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype, int32_t form,

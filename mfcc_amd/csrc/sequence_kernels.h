@@ -96,8 +96,9 @@ __device__ inline int64_t scalar(int64_t v) {
   return (int64_t)((uint64_t)(uint32_t)scalar((int)v) | (uint64_t)(uint32_t)scalar((int)(v >> 32)) << 32);
 }
 
-// What a thread works on.  Threads behind the last slot or column group are doubles of others: they compute and write the
-// same values, so that no access to rows needs a predicate as long as a tile is full.
+// What a thread works on.  Threads behind the last slot or column group are doubles of others: in full tiles they compute and
+// write the same values, so that no access to rows needs a predicate. (y may be x: what a thread leaves in LDS before the barrier
+// depends on all rows it has loaded, and rows are written behind the barrier.) Elsewhere only owners write.
 struct Seat {
   int64_t u;           // sequence
   Span s;
@@ -105,6 +106,7 @@ struct Seat {
   int piece, tile, tiles, full;  // the tiles [tile, tiles) of the sequence, those below `full` without a missing row
   bool on;             // there is such a sequence
   bool there;          // the workgroup has something to do
+  bool own;            // not a double
 };
 template <int V>
 __device__ inline Seat seat_of(const Batch& b, const Split& w) {
@@ -116,7 +118,10 @@ __device__ inline Seat seat_of(const Batch& b, const Split& w) {
   t.there = at < w.blocks;
   t.piece = at - block * w.pieces;
   t.slot = threadIdx.x / w.cb;
-  t.cg = min((int)threadIdx.x - t.slot * w.cb, w.groups - 1 - column_block * w.cb);
+  t.cg = (int)threadIdx.x - t.slot * w.cb;
+  const int groups = w.groups - column_block * w.cb;
+  t.own = t.slot < w.seqs * w.per && t.cg < groups;
+  t.cg = min(t.cg, groups - 1);
   if (t.slot >= w.seqs * w.per) t.slot = 0;
   t.col = (column_block * w.cb + t.cg) * V;
   const int tile_rows = w.per * kSlotRows;
@@ -408,11 +413,10 @@ __global__ void __launch_bounds__(kSeqThreads, 4) gated_scan_kernel(const Batch 
           carry[v] = fmaf(f.x, carry[v], f.y);
         }
     } else {
-      __syncthreads();   // doubles have read their rows: y may be x
 #pragma unroll
       for (int v = 0; v < V; ++v) h[v] = carry[v], carry[v] = fmaf(A[v], carry[v], X[v]);
     }
-    if (ck && t.sub == 0 && k > 0)
+    if (ck && t.own && t.sub == 0 && k > 0)
 #pragma unroll
       for (int v = 0; v < V; ++v) ck[(int64_t)tile * b.ncol + v] = h[v];
     const uint32_t to = here(fy.off);
@@ -420,7 +424,7 @@ __global__ void __launch_bounds__(kSeqThreads, 4) gated_scan_kernel(const Batch 
     for (int r = 0; r < R; ++r) {
 #pragma unroll
       for (int v = 0; v < V; ++v) h[v] = fmaf(a[r][v], h[v], x1[r][v]);
-      if (FULL || r < k) store_pack<AL, V>(row_at<FULL>(fy, t, w, tile, r, to), h);
+      if (FULL || (t.own && r < k)) store_pack<AL, V>(row_at<FULL>(fy, t, w, tile, r, to), h);
     }
   };
 
@@ -450,10 +454,10 @@ __global__ void __launch_bounds__(kSeqThreads, 4) gated_scan_kernel(const Batch 
   }
   // the state behind the last row, from the thread that walked it: the very value that y rounds
   const int lead = t.n > 0 ? (t.n - 1) / R % w.per : 0;
-  if (t.on && q.last && t.sub == lead && (t.n > 0 ? t.tile < t.tiles && t.tiles * w.per * R >= t.n : t.piece == 0))
+  if (t.on && t.own && q.last && t.sub == lead && (t.n > 0 ? t.tile < t.tiles && t.tiles * w.per * R >= t.n : t.piece == 0))
 #pragma unroll
     for (int v = 0; v < V; ++v) q.last[end + v] = t.n > 0 ? h[v] : carry[v];
-  if (t.on && b.steps) zero_behind<AL, V>(y, b, w, t);
+  if (t.on && t.own && b.steps) zero_behind<AL, V>(y, b, w, t);
 }
 
 // Gradient.  With e_t = a_t delta_t, delta_t = gy_t + e_{t+1}, the way back is a composition of maps e -> A (gy + e) with the
@@ -555,7 +559,7 @@ __global__ void __launch_bounds__(kSeqThreads, 2) gated_scan_backward_kernel(con
           e[v] = a[r][v] * d;
           dg[v] = SIG ? e[v] * na[r][v] * (hp[r][v] - (float)in.x[r].v[v]) : d * hp[r][v];
         }
-        if (FULL || r < k) {
+        if (FULL || (t.own && r < k)) {
           store_pack<AL, V>(row_at<FULL>(fgx, t, w, tile, r, to_x), dx);
           store_pack<AL, V>(row_at<FULL>(fgg, t, w, tile, r, to_g), dg);
         }
@@ -584,10 +588,10 @@ __global__ void __launch_bounds__(kSeqThreads, 2) gated_scan_backward_kernel(con
       work(std::true_type(), in, tile);
     }
   }
-  if (t.on && q.gh0 && t.sub == 0 && t.piece == 0)
+  if (t.on && t.own && q.gh0 && t.sub == 0 && t.piece == 0)
 #pragma unroll
     for (int v = 0; v < V; ++v) q.gh0[end + v] = carry[v];
-  if (t.on && b.steps) {
+  if (t.on && t.own && b.steps) {
     zero_behind<AL, V>(gx, b, w, t);
     zero_behind<AL, V>(gg, b, w, t);
   }
@@ -791,7 +795,7 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batc
       for (int v = 0; v < V; ++v) mean[v] = (double)base[v] + off[v];
       weight = fma(a.tile_decay, weight, a.tile_grown);   // behind a last tile with missing rows it is not used
     } else {
-      __syncthreads();   // 1 / w; and doubles have read their rows: y may be x
+      __syncthreads();   // 1 / w
 #pragma unroll
       for (int v = 0; v < V; ++v) m[v] = base[v], q[v] = square[v];
     }
@@ -812,7 +816,7 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batc
         m[v] = FULL || r < k ? mn : m[v];
         q[v] = FULL || r < k ? qn : q[v];
       }
-      if (FULL || r < k) store_pack<AL, V>(row_at<FULL>(fy, t, w, tile, r, to), o);
+      if (FULL || (t.own && r < k)) store_pack<AL, V>(row_at<FULL>(fy, t, w, tile, r, to), o);
     }
   };
 
@@ -874,7 +878,7 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batc
   }
   // the state behind the last row, from the thread that walked it
   const int lead = t.n > 0 ? (t.n - 1) / R % w.per : 0;
-  if (t.on && a.state_out && t.sub == lead && (t.n > 0 ? t.tile < t.tiles && t.tiles * w.per * R >= t.n : t.piece == 0)) {
+  if (t.on && t.own && a.state_out && t.sub == lead && (t.n > 0 ? t.tile < t.tiles && t.tiles * w.per * R >= t.n : t.piece == 0)) {
     auto entered = [&](int64_t i) { return a.state_in ? a.state_in[state + i] : 0.0f; };   // passes through where there are no rows
     if (t.col == 0) a.state_out[state] = t.n > 0 ? last_weight : entered(0);
 #pragma unroll
@@ -883,7 +887,7 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batc
       a.state_out[state + 1 + b.ncol + t.col + v] = t.n > 0 ? q[v] : entered(1 + b.ncol + t.col + v);
     }
   }
-  if (t.on && b.steps) zero_behind<AL, V>(y, b, w, t);
+  if (t.on && t.own && b.steps) zero_behind<AL, V>(y, b, w, t);
 }
 
 // ---- dropout --------------------------------------------------------------------------------------------

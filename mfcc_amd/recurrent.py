@@ -83,8 +83,9 @@ def _rows(t):
 
 
 def _check(t, name, like=None, dtypes=_ROWS):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes or (t.stride(-1) != 1 and t.shape[-1] > 1):
-        raise ValueError(f"{name} must be a device tensor of " + " / ".join(str(d).replace("torch.", "") for d in dtypes)
+    if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes or t.dim() < 2
+            or (t.stride(-1) != 1 and t.shape[-1] > 1)):
+        raise ValueError(f"{name} must be a device tensor of rows of " + " / ".join(str(d).replace("torch.", "") for d in dtypes)
                          + " with unit column stride")
     if like is not None and (t.shape != like.shape or t.dtype != like.dtype):
         raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype}, expected {tuple(like.shape)} {like.dtype}")

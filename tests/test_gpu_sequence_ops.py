@@ -691,3 +691,109 @@ def test_streaming_with_running_norm(M):
     t.push(torch.from_numpy(audio[:, :4000]).cuda())
     t.reset()
     assert torch.equal(t.push(torch.from_numpy(audio).cuda()), parts[0])
+
+
+# --------------------------------------------------------------------------
+# the corners of the division over workgroups
+# --------------------------------------------------------------------------
+@pytest.mark.parametrize("counts,d", [([600, 13, 590] + [450] * 13, 512), ([700, 0, 3, 650], 257), ([30] * 40, 130), ([3, 20, 17, 1, 24] * 9, 5)])
+def test_scan_divisions(M, counts, d):
+    """Narrower column blocks for few sequences, several short sequences to a workgroup, several column blocks."""
+    check_scan(M, counts, d, torch.float32, "sigmoid", seed=d)
+    check_scan(M, counts, d, torch.bfloat16, "decay", reverse=True, seed=d, h0=False)
+
+
+def test_norm_many_sequences(M):
+    """So many sequences that workgroups take half the threads."""
+    rng = np.random.default_rng(5)
+    check_norm(M, [120] + rng.integers(0, 21, size=2100).tolist(), 39, 0.98, seed=2)
+
+
+@pytest.mark.parametrize("n,k,d", [(64, 1, 39), (200, 3, 39), (40, 8, 13), (500, 5, 2)])
+def test_short_sequences_in_place(M, n, k, d):
+    """One slot of time to a sequence; threads without a slot of their own must not disturb the rows of others."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    x, g = torch.randn(n, k, d, generator=gen, device="cuda"), torch.rand(n, k, d, generator=gen, device="cuda")
+    st = M.running_norm(torch.randn(n, 50, d, generator=gen, device="cuda"))[1]
+    want_y, want_last = M.gated_scan(x, g, form="sigmoid")
+    want_n, want_s = M.running_norm(x, state=st)
+    for _ in range(20):
+        a, b = x.clone(), x.clone()
+        y, last = M.gated_scan(a, g, form="sigmoid", out=a)
+        z, s = M.running_norm(b, state=st, out=b)
+        assert torch.equal(a, want_y) and torch.equal(last, want_last) and torch.equal(b, want_n) and torch.equal(s, want_s)
+    # y over the gates instead
+    c = g.clone()
+    M.gated_scan(x, c, form="sigmoid", out=c)
+    assert torch.equal(c, want_y)
+
+
+def test_rows_far_apart(M):
+    """Row strides at which a tile spans more than 4 GiB."""
+    n, d, ld = 220, 40, 10_500_000
+    big = torch.empty(n * ld, device="cuda")
+    far = big.as_strided((n, d), (ld, 1))
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x, g, gy = (torch.randn(n, d, generator=gen, device="cuda") for _ in range(3))
+    far.copy_(x)
+    for reverse in (False, True):
+        a, b = x.clone().requires_grad_(True), g.clone().requires_grad_(True)
+        y, last = M.gated_scan(a, b, [200, 20], form="sigmoid", reverse=reverse)
+        want = torch.autograd.grad((y, last), (a, b), (gy, torch.ones_like(last)))
+        c, e = far.detach().requires_grad_(True), g.clone().requires_grad_(True)
+        y2, last2 = M.gated_scan(c, e, [200, 20], form="sigmoid", reverse=reverse)
+        got = torch.autograd.grad((y2, last2), (c, e), (gy, torch.ones_like(last)))
+        assert torch.equal(y, y2) and torch.equal(last, last2) and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    z, s = M.running_norm(x, [200, 20])
+    z2, s2 = M.running_norm(far, [200, 20], out=far)
+    assert z2 is far and torch.equal(z, far) and torch.equal(s, s2)
+    far.copy_(x)
+    for per in ("element", "frame", "sequence"):
+        assert torch.equal(M.feature_dropout(far, 0.4, 5, per=per, frame_counts=[200, 20]), M.feature_dropout(x, 0.4, 5, per=per, frame_counts=[200, 20]))
+    del big, far, z2, c, got
+
+
+def test_more_than_2_31_values(M):
+    n, d = 70000, 32768
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(n, d, generator=gen, device="cuda", dtype=torch.float16)
+    g = torch.full((1, d), 3.0, device="cuda", dtype=torch.float16).expand(n, d)
+    y, last = M.gated_scan(x, g, form="sigmoid")
+    cols = [0, 1, 12345, d - 1]
+    xs = host(x[:, cols])
+    out, mag = sequence(xs, np.full_like(xs, 3.0), np.zeros(4), "sigmoid", False)
+    close(y[:, cols], out[0], mag[0], torch.float16, memory(np.array([3.0]), "sigmoid", n), "y")
+    close(last[0, cols], out[1], mag[1], torch.float32, memory(np.array([3.0]), "sigmoid", n), "last")
+    M.feature_dropout(x, 0.3, 21, step=2, out=y)
+    rows = [0, 1, 65535, n - 1]
+    e = np.array(rows, dtype=np.uint64)[:, None] * np.uint64(d) + np.arange(d, dtype=np.uint64)
+    keep = fields(e, 2, 21) >= int(round(0.3 * 65536))
+    got, src = host(y[rows]), host(x[rows])
+    assert np.array_equal(got == 0, ~keep | (src == 0))
+    ref = src * keep * 65536 / (65536 - int(round(0.3 * 65536)))
+    assert (np.abs(got - ref) <= (2 * U + HALF[torch.float16]) * np.abs(ref) + TINY[torch.float16]).all()
+    del x, y
+
+
+def test_not_rows(M):
+    v = torch.zeros(8, device="cuda")
+    for f in (lambda: M.gated_scan(v, v), lambda: M.gated_scan(v[0], v[0]), lambda: M.running_norm(v), lambda: M.feature_dropout(v, 0.5, 1),
+              lambda: M.gated_scan_step(v, v, v), lambda: M.gated_scan(None, v), lambda: M.gated_scan(torch.zeros(3, 0, device="cuda"), torch.zeros(3, 0, device="cuda"))):
+        with pytest.raises(ValueError):
+            f()
+
+
+def test_gradient_at_another_stream(M):
+    """The backward pass runs on the stream of the forward pass, with the caller ordering the streams as usual."""
+    x, g = torch.randn(5000, 64, device="cuda", requires_grad=True), torch.randn(5000, 64, device="cuda", requires_grad=True)
+    y, last = M.gated_scan(x, g, form="sigmoid")
+    want = torch.autograd.grad(y.sum() + last.sum(), (x, g))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y, last = M.gated_scan(x, g, form="sigmoid")
+        loss = y.sum() + last.sum()
+    torch.cuda.current_stream().wait_stream(side)
+    got = torch.autograd.grad(loss, (x, g))
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
