@@ -37,11 +37,6 @@ __device__ inline Span span_of(const Batch& b, int64_t u) {
   const int64_t lo = b.off[u], n = b.off[u + 1] - lo;
   return b.steps ? Span{0, n < b.steps ? n : b.steps} : Span{lo, n};
 }
-template <typename T>
-__device__ inline T* row_base(const Rows<T>& r, const Batch& b, int64_t u, const Span& s) {
-  return r.p + (b.steps ? u * r.ss : 0) + (s.first + (b.reverse ? s.n - 1 : 0)) * r.rs;
-}
-
 // ---- the division of a batch over threads ----------------------------------------------------------
 // A workgroup owns `seqs` sequences and `cb` groups of V neighbouring columns; its threads are (time slot, column group)
 // pairs, `per` slots to a sequence.  A tile is per * R rows: a thread keeps the R x V values of its slot in registers,
@@ -627,7 +622,8 @@ __global__ void __launch_bounds__(256) gated_scan_step_kernel(int64_t n, int nco
 // join is shared by R values only).
 struct NormArgs {
   double decay, log_decay;      // log_decay = log1p(decay - 1)
-  double slot_decay, slot_grown, tile_decay, tile_grown;   // decay^k and g(k) of a slot and of a tile
+  // decay^k and g(k) of a slot, a tile, a slot's run of a piece, a piece
+  double slot_decay, slot_grown, tile_decay, tile_grown, run_decay, run_grown, piece_decay, piece_grown;
   float eps, decayed[kSlotRows], grown[kSlotRows], inv_grown[kSlotRows];   // decay^k, g(k), 1 / g(k) for k = 1 .. R
   int center_only;
   const float* state_in;
@@ -694,8 +690,7 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_pieces_kernel(con
   for (int v = 0; v < V; ++v) runs[(t.slot * V + v) * w.cb + t.cg] = make_float2(m[v], q[v]);
   __syncthreads();
   if (t.sub == 0) {
-    double l, g;
-    weights_of(a, run, l, g);
+    double l = a.run_decay, g = a.run_grown;
     float ws = 0.0f, ms[V] = {}, qs[V] = {};
     for (int s = 0; s < w.per; ++s) {
       const int k = min(max(t.n - first - s * run, 0), run);
@@ -825,11 +820,11 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batc
     int tile = t.tile;
     load_rows<false, AL>(in, fx, t, w, tile);
     if (t.piece > 0) {
-      // the pieces before this one: each slot joins a run of them, the slots meet in LDS
-      double l, g, lr, gr;
-      weights_of(a, w.piece_tiles * w.per * R, l, g);
+      // the pieces before this one, all of them full: each slot joins a run of them, the slots meet in LDS with the weights of
+      // their runs in 64 bits
       const int run = (t.piece + w.per - 1) / w.per, lo = t.sub * run, hi = min(lo + run, t.piece);
       const float2* p = a.runs + (t.u * w.pieces + lo) * b.ncol + t.col;
+      double run_decay = 1.0, run_grown = 0.0;
       float sum = 0.0f;
 #pragma unroll 8
       for (int i = lo; i < hi; ++i, p += b.ncol) {
@@ -837,26 +832,34 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batc
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           wn = sum;
-          norm_join(wn, m[v], q[v], (float)l, (float)g, p[v].x, p[v].y);
+          norm_join(wn, m[v], q[v], (float)a.piece_decay, (float)a.piece_grown, p[v].x, p[v].y);
         }
         sum = wn;
+        run_decay *= a.piece_decay;
+        run_grown = fma(a.piece_decay, run_grown, a.piece_grown);
       }
+      double* const weights = (double*)joins;   // two of every slot
 #pragma unroll
       for (int v = 0; v < V; ++v) runs[(t.slot * V + v) * w.cb + t.cg] = make_float2(m[v], q[v]);
+      if (t.cg == 0) weights[2 * t.slot] = run_decay, weights[2 * t.slot + 1] = run_grown;
       __syncthreads();
-      weights_of(a, (double)run * w.piece_tiles * w.per * R, lr, gr);
+      float off[V] = {}, base[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) base[v] = (float)mean[v], off[v] = (float)(mean[v] - base[v]);
       for (int s = 0; s < w.per && s * run < t.piece; ++s) {
-        if (t.piece - s * run < run) weights_of(a, (double)(t.piece - s * run) * w.piece_tiles * w.per * R, lr, gr);
-        const double old = lr * weight, f = gr / (old + gr);
+        const double old = weights[2 * s] * weight, g = weights[2 * s + 1];
+        const float l = (float)weights[2 * s], f = old > 0.0 ? (float)g * __builtin_amdgcn_rcpf((float)(old + g)) : 1.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float2 e = runs[(s * V + v) * w.cb + t.cg];
-          const double d = e.x - mean[v];
-          mean[v] = fma(d, f, mean[v]);
-          square[v] = (float)(lr * square[v] + e.y + d * d * old * f);
+          const float d = e.x - base[v] - off[v];
+          off[v] = fmaf(d, f, off[v]);
+          square[v] = fmaf(l, square[v], fmaf(d * d, (float)old * f, e.y));
         }
-        weight = old + gr;
+        weight = old + g;
       }
+#pragma unroll
+      for (int v = 0; v < V; ++v) mean[v] = (double)base[v] + off[v];
       __syncthreads();
     }
     for (; tile + 1 < t.full; ++tile) {

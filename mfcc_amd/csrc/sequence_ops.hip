@@ -55,7 +55,8 @@ int check_rows(const char* who, const char* name, const mfcc_rows* r, const Shap
 // 17.1 (38.8).  32 sequences of up to 700 rows (11 tiles, 4 pieces would fill the card) 18.9 us whole, 28 in pieces.
 constexpr int64_t kFewBlocks = 256, kManyTiles = 10, kManyPieces = 5, kTargetBlocks = 512, kPieceTiles = 2;
 
-// Workgroups of half the threads for the normalisation where there are many: half the slots to join a tile.
+// Workgroups of half the threads for the normalisation where there are many: half the slots to join a tile (10000 sequences of
+// 299 rows of 39: 272 us with 512 threads, 228 with 256; 200 sequences of up to 1200 rows of 257, 1000 workgroups: 57 and 61).
 constexpr int64_t kManyBlocks = 2048;
 
 // How workgroups divide sequences, columns and time.  It depends on the shape of the batch alone, so that the backward
@@ -288,6 +289,8 @@ int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_ste
   };
   weights(mfcc::kSlotRows, &a.slot_decay, &a.slot_grown);
   weights(c.tile_rows, &a.tile_decay, &a.tile_grown);
+  weights((double)c.w.piece_tiles * mfcc::kSlotRows, &a.run_decay, &a.run_grown);
+  weights((double)c.w.piece_tiles * c.tile_rows, &a.piece_decay, &a.piece_grown);
   for (int r = 0; r < mfcc::kSlotRows; ++r) {
     double l, g;
     weights(r + 1, &l, &g);
