@@ -28,7 +28,7 @@ struct Batch {
   int32_t reverse;
 };
 
-// Rows of sequence u and where its first visited row lies (sign: the direction of the visit).
+// Rows of sequence u, and the row of the array that its first one is.
 struct Span {
   int64_t first, n;
 };
@@ -48,7 +48,8 @@ constexpr int kSlotRows = 8;   // R: composing costs per / R steps a value, regi
 
 // Where the sequences and columns are too few for the card, a sequence is also cut into `pieces` of `piece_tiles` tiles, a
 // workgroup each: a first kernel composes every piece into one entry of a workspace, the second one composes the entries before its
-// piece and goes on from there (the rows are read twice, mostly from the caches the second time).
+// piece and goes on from there. The rows are read twice; a single pass would have each workgroup hold its rows while it waits for
+// the entries of all before it.
 struct Split {
   int32_t groups, cb;    // column groups of a row, of a workgroup
   int32_t column_blocks; // workgroups to a row
@@ -72,6 +73,7 @@ __device__ inline void load_pack(Pack<T, V>& r, const T* p) {
     for (int i = 0; i < V; ++i) r.v[i] = p[i];
   }
 }
+// The one rounding to the type of the rows: everything before it is 32 or 64 bits wide.
 template <bool AL, int V, typename T>
 __device__ inline void store_pack(T* p, const float* f) {
   if constexpr (AL || V == 1) {
@@ -240,7 +242,10 @@ __device__ inline void load_run(Pack<T, V> (&r)[kSlotRows], const RunLane<S>& l,
 
 // ---- gated recurrence -----------------------------------------------------------------------------
 // h_t = a_t h_{t-1} + b_t is a composition of maps h -> A h + X: a run of rows is one such map, and maps of neighbouring
-// runs join to (A2 A1, A2 X1 + X2).  Bound: HBM, 3 values moved a value forward and 5 backward.
+// runs join to (A2 A1, A2 X1 + X2).  Bound: HBM, 3 values moved a value forward and 5 backward.  512 sequences of 1024 rows of 512
+// bfloat16: forward 5.1 TB/s, backward 4.9 (a copy of that size 5.3); 10000 of 300 rows of 39 floats 5.4 and 5.1; 2048 of 512 rows of
+// 257 floats 4.4 and 4.0 (column blocks share cache lines).  A batch of 64 sequences of 100 to 1500 rows of 1024 bfloat16
+// 86 + 125 us, 4.1 TB/s: at the end the tiles of the longest ones follow each other with the card half empty.
 
 // a = 1 / (1 + e) and 1 - a = e a from e = exp(-g), neither by a difference.  g is held above -87 so that e stays finite (a is
 // 2^-125 there; a NaN stays one).  The hardware exponential and reciprocal are good to one unit in the last place, and the
@@ -269,7 +274,8 @@ struct ScanRows {
 };
 
 // The map of every piece: forward h -> A h + X from (x, gate), backward e -> A e + E from (gate, grad_y). A slot takes a contiguous
-// run of the piece, so that the threads meet once.
+// run of the piece, so that the threads meet once.  Bound: HBM, 2 values read a value; 360000 rows of 256 float16: both kernels
+// 205 us for 921 MB, 4.5 TB/s (whole, without pieces: 9.6 ms).
 template <typename T, int V, bool AL, bool SIG, bool BACK>
 __global__ void __launch_bounds__(kSeqThreads, 4) gated_scan_pieces_kernel(const Batch b, const Split w, const Rows<const T> x,
                                                                            const Rows<const T> g, const ScanPtrs q) {
@@ -458,6 +464,8 @@ __global__ void __launch_bounds__(kSeqThreads, 4) gated_scan_kernel(const Batch 
 // Gradient.  With e_t = a_t delta_t, delta_t = gy_t + e_{t+1}, the way back is a composition of maps e -> A (gy + e) with the
 // same products of gates, from the last tile to the first; the states h_{t-1} that dgate needs are walked
 // again from the checkpoint of the tile.
+// 152 to 197 registers of V = 2 leave 2 waves a SIMD; bounded to 128 they spill, and the step on 64 x 1500 x 1024 takes 510 us
+// instead of 213.
 template <typename T, int V>
 struct ScanGradRows {
   Pack<T, V> x[kSlotRows], g[kSlotRows], d[kSlotRows];
@@ -592,6 +600,8 @@ __global__ void __launch_bounds__(kSeqThreads, 2) gated_scan_backward_kernel(con
   }
 }
 
+// One step of live sequences, a thread to a value: 64 x 512 floats are 0.7 MB, the launch is what it costs (4.7 us each in a
+// captured sequence of them).
 template <typename T, bool SIG>
 __global__ void __launch_bounds__(256) gated_scan_step_kernel(int64_t n, int ncol, const T* x, int64_t x_ld, const T* g, int64_t g_ld,
                                                               const float* hin, float* hout, T* y, int64_t y_ld) {
@@ -618,8 +628,9 @@ __global__ void __launch_bounds__(256) gated_scan_step_kernel(int64_t n, int nco
 // point of w the roundings of 32 bits have one sign: 7e-6 of w off after 20000 rows at decay 0.995), and f and decay^k w f are
 // computed once per slot. The mean that enters a tile is carried in 64 bits and the tile composes 32-bit deviations from it: a
 // cumulative mean of n rows would otherwise collect sqrt(n) / 4 units in the last place.
-// Bound: HBM, one value read and one written; about 35 instructions a value, so slots are few where sequences are many (every
-// join is shared by R values only).
+// Bound: HBM, one value read and one written, closely followed by the vector pipe: 31 instructions a value in full tiles, 47 with the
+// ends of 299 rows (68 % of the cycles of 10000 sequences of 39 columns: 228 us, 4.1 TB/s), so slots are few where sequences are
+// many (every join is shared by R values only). One hour of 39 columns, cumulative: 12 us for the pieces, 33 us for the rows.
 struct NormArgs {
   double decay, log_decay;      // log_decay = log1p(decay - 1)
   // decay^k and g(k) of a slot, a tile, a slot's run of a piece, a piece
@@ -931,8 +942,8 @@ struct Dropout {
 
 // per = element: a thread takes the 8 consecutive elements of one block. FLAT: rows back to back in both arrays and 16-byte
 // aligned, an element is its number. Otherwise (row, column) of the first one by division, then step by step.
-// Bound: HBM, read once and written once (20000 x 4369 bfloat16, both passes: see the table of measurements); the 20 wide products
-// of a block are shared by 8 elements.
+// Bound: HBM, read once and written once: 20000 x 4369 bfloat16 75 us a pass, 4.6 TB/s; the 20 wide products of a block are shared
+// by 8 elements (an element to a thread: 290 us).
 template <typename T, bool FLAT>
 __global__ void __launch_bounds__(256) dropout_element_kernel(const Batch b, int64_t n_rows, const Dropout d, const Rows<const T> x,
                                                               const Rows<T> y) {
@@ -966,7 +977,8 @@ __global__ void __launch_bounds__(256) dropout_element_kernel(const Batch b, int
 }
 
 // per = frame or sequence: a thread takes V columns of the 8 rows of one group of row numbers; its block decides the 8 rows, or
-// its column for as long as the sequence lasts.
+// its column for as long as the sequence lasts.  64 utterances of 39 floats (7.6 MB): 6 us, most of it the launch and the search for
+// the sequence of a row.
 template <typename T, int V, bool FRAME>
 __global__ void __launch_bounds__(256) dropout_rows_kernel(const Batch b, const Split w, int64_t n_rows, const Dropout d,
                                                            const Rows<const T> x, const Rows<T> y) {

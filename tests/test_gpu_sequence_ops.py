@@ -797,3 +797,33 @@ def test_gradient_at_another_stream(M):
     got = torch.autograd.grad(loss, (x, g))
     torch.cuda.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_padding_is_not_read_and_audio_layouts(M):
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    lens = [40, 0, 300, 17, 299]
+    for reverse in (False, True):
+        x, g, gy = (torch.randn(5, 300, 39, generator=gen, device="cuda") for _ in range(3))
+        runs = []
+        for fill in (0.0, float("nan")):
+            a, b, c = x.clone(), g.clone(), gy.clone()
+            for u, n in enumerate(lens):
+                for t in (a, b, c):
+                    t[u, n:] = fill
+            z, s = M.running_norm(a, lens)
+            a.requires_grad_(True), b.requires_grad_(True)
+            y, last = M.gated_scan(a, b, lens, form="sigmoid", reverse=reverse)
+            runs.append((z, s, y.detach(), last.detach()) + torch.autograd.grad(y, (a, b), c))
+        for p, q in zip(*runs):
+            assert torch.equal(p, q) and torch.isfinite(p).all()
+    # the layout that cut the audio also tells the sequences of its rows
+    fe = M.MFCC("self5")
+    rng = np.random.default_rng(1)
+    lengths = [16000, 4000, 23456]
+    audio = torch.from_numpy(np.clip(rng.standard_normal(sum(lengths)) * 3000, -32768, 32767).astype(np.int16)).cuda()
+    lay = fe.layout(lengths)
+    feats = fe.forward(audio, lay)
+    counts = np.diff(lay.frame_offsets)
+    assert torch.equal(M.running_norm(feats, lay)[0], M.running_norm(feats, counts)[0])
+    assert torch.equal(M.gated_scan(feats, torch.sigmoid(feats), lay)[0], M.gated_scan(feats, torch.sigmoid(feats), torch.from_numpy(counts))[0])
+    assert torch.equal(M.feature_dropout(feats, 0.5, 1, per="sequence", frame_counts=lay), M.feature_dropout(feats, 0.5, 1, per="sequence", frame_counts=counts))
