@@ -964,31 +964,54 @@ __global__ void __launch_bounds__(256) dropout_element_kernel(const Batch b, int
     for (int i = 0; i < 8 / V; ++i) *(Pack<T, V>*)(y.p + e0 + i * V) = r[i];
     return;
   }
-  const int64_t row = e0 / b.ncol;
-  int64_t c = e0 - row * b.ncol, u = b.steps ? row / b.steps : 0, t = row - u * b.steps;
-  for (int i = 0; i < 8 && e0 + i < total; ++i) {
-    const float v = (float)x.p[u * x.ss + t * x.rs + c] * d.scale;
-    y.p[u * y.ss + t * y.rs + c] = gone >> i & 1 ? (T)0.0f : (T)v;
-    if (++c == b.ncol) {
-      c = 0;
-      if (++t == b.steps) t = 0, ++u;   // packed rows: steps is 0, t never
-    }
+  const int64_t row = total < ((int64_t)1 << 32) ? (int64_t)((uint32_t)e0 / (uint32_t)b.ncol) : e0 / b.ncol;
+  int64_t u = 0, t = row;
+  if (b.steps) {
+    u = n_rows < ((int64_t)1 << 32) ? (int64_t)((uint32_t)row / (uint32_t)b.steps) : row / b.steps;
+    t = row - u * b.steps;
   }
+  int c = (int)(e0 - row * b.ncol);
+  const int k = (int)min((int64_t)8, total - e0);
+  // all loads first; behind the last element they repeat it
+  int64_t to[8];
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = (float)x.p[u * x.ss + t * x.rs + c];
+    to[i] = u * y.ss + t * y.rs + c;
+    const bool more = i + 1 < k, wrap = more && c + 1 == b.ncol, next = wrap && t + 1 == b.steps;   // packed rows: steps is 0
+    c = wrap ? 0 : more ? c + 1 : c;
+    t = next ? 0 : wrap ? t + 1 : t;
+    u = next ? u + 1 : u;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < k) y.p[to[i]] = gone >> i & 1 ? (T)0.0f : (T)(v[i] * d.scale);
 }
 
-// per = frame or sequence: a thread takes V columns of the 8 rows of one group of row numbers; its block decides the 8 rows, or
-// its column for as long as the sequence lasts.  64 utterances of 39 floats (7.6 MB): 6 us, most of it the launch and the search for
-// the sequence of a row.
-template <typename T, int V, bool FRAME>
-__global__ void __launch_bounds__(256) dropout_rows_kernel(const Batch b, const Split w, int64_t n_rows, const Dropout d,
+// per = frame or sequence: a thread takes V columns of `runs` groups of 8 rows, loading a group at a time.  A block decides 8 rows:
+// it is made once for the workgroup (LDS); or 8 columns for as long as the sequence lasts: a thread makes it again where the sequence
+// changes.  More groups a thread share the search for the first row's sequence and the blocks, fewer fill the card.
+// LINEAR: row number times row stride is the address, padded batches included.
+// Bound: HBM, read once and written once: 256 x 1024 rows of 512 float16 5.0 to 5.2 TB/s; 39 columns of bfloat16 3.1 to 3.5, two
+// bytes a lane.  64 utterances of 39 floats: 5 us, the launch and the search.
+constexpr int kDropRuns = 8;
+template <typename T, int V, bool FRAME, bool LINEAR>
+__global__ void __launch_bounds__(256) dropout_rows_kernel(const Batch b, const Split w, int runs, int64_t n_rows, const Dropout d,
                                                            const Rows<const T> x, const Rows<T> y) {
+  __shared__ uint32_t rows_gone[256 * kDropRuns];
   const int slot = threadIdx.x / w.cb, group = blockIdx.y * w.cb + (threadIdx.x - slot * w.cb);
-  const int64_t r0 = ((int64_t)blockIdx.x * w.per + slot) * 8;
+  const int64_t first = (int64_t)blockIdx.x * w.per * runs, step = (int64_t)d.at();   // the first group of 8 rows of the workgroup
+  if (FRAME) {
+    for (int i = threadIdx.x; i < w.per * runs; i += 256) rows_gone[i] = philox_dropped((uint64_t)(first + i), step, d.seed, d.threshold);
+    __syncthreads();
+  }
+  const int64_t r0 = (first + slot * runs) * 8;
   if (slot >= w.per || group >= w.groups || r0 >= n_rows) return;
-  const int col = group * V, k = (int)min((int64_t)8, n_rows - r0);
+  const int col = group * V;
   int64_t u = 0, end = n_rows;   // the sequence of a row, the first row behind it
   if (b.steps) {
-    u = r0 / b.steps;
+    u = n_rows < ((int64_t)1 << 32) ? (int64_t)((uint32_t)r0 / (uint32_t)b.steps) : r0 / b.steps;
     end = (u + 1) * b.steps;
   } else if (!FRAME && b.off) {   // the last u with off[u] <= r0
     int64_t hi = b.n_seq;
@@ -998,27 +1021,37 @@ __global__ void __launch_bounds__(256) dropout_rows_kernel(const Batch b, const 
     }
     end = b.off[u + 1];
   }
-  const int64_t step = d.at();
   const int wide = (b.ncol + 7) / 8;
   auto columns = [&]() { return philox_dropped((uint64_t)u * wide + col / 8, step, d.seed, d.threshold) >> (col & 7); };
-  uint32_t gone = FRAME ? philox_dropped((uint64_t)(r0 >> 3), step, d.seed, d.threshold) : columns();
-  const bool split = b.steps || (!FRAME && b.off);
+  uint32_t gone = FRAME ? 0 : columns();
+  const bool split = FRAME ? !LINEAR : b.steps || b.off;
+  for (int g = 0; g < runs; ++g) {
+    const int64_t r = r0 + g * 8;
+    const int k = (int)min((int64_t)8, n_rows - r);
+    if (k <= 0) return;
+    Pack<T, V> v[8];
+    if (LINEAR) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (i >= k) break;
-    const int64_t r = r0 + i;
-    if (split && r >= end) {
-      do end = b.steps ? end + b.steps : b.off[++u + 1]; while (r >= end);
-      if (b.steps) u = end / b.steps - 1;
-      if (!FRAME) gone = columns();
+      for (int i = 0; i < 8; ++i) load_pack<true>(v[i], x.p + (r + min(i, k - 1)) * x.rs + col);
     }
-    const int64_t t = b.steps ? r - u * b.steps : r;
-    Pack<T, V> v;
-    load_pack<true>(v, x.p + (b.steps ? u * x.ss : 0) + t * x.rs + col);
-    float f[V];
+    if (FRAME) gone = rows_gone[slot * runs + g];
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = gone >> (FRAME ? i : j) & 1 ? 0.0f : (float)v.v[j] * d.scale;
-    store_pack<true, V>(y.p + (b.steps ? u * y.ss : 0) + t * y.rs + col, f);
+    for (int i = 0; i < 8; ++i) {
+      if (i >= k) break;
+      if (split && r + i >= end) {
+        do end = b.steps ? end + b.steps : b.off[++u + 1]; while (r + i >= end);
+        if (b.steps) u = end / b.steps - 1;
+        if (!FRAME) gone = columns();
+      }
+      const int64_t at = LINEAR ? 0 : u * x.ss + (r + i - u * b.steps) * x.rs;
+      const int64_t to = LINEAR ? (r + i) * y.rs : u * y.ss + (r + i - u * b.steps) * y.rs;
+      Pack<T, V> f;
+      if (LINEAR) f = v[i]; else load_pack<true>(f, x.p + at + col);
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = gone >> (FRAME ? i : j) & 1 ? 0.0f : (float)f.v[j] * d.scale;
+      store_pack<true, V>(y.p + to + col, o);
+    }
   }
 }
 

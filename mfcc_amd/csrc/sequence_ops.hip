@@ -58,6 +58,7 @@ constexpr int64_t kFewBlocks = 256, kManyTiles = 10, kManyPieces = 5, kTargetBlo
 // Workgroups of half the threads for the normalisation where there are many: half the slots to join a tile (10000 sequences of
 // 299 rows of 39: 272 us with 512 threads, 228 with 256; 200 sequences of up to 1200 rows of 257, 1000 workgroups: 57 and 61).
 constexpr int64_t kManyBlocks = 2048;
+constexpr int kWideBlock = 40, kManySlots = 12;
 
 // How workgroups divide sequences, columns and time.  It depends on the shape of the batch alone, so that the backward
 // pass finds its checkpoints whatever the alignment of its arrays.
@@ -68,8 +69,6 @@ struct Grid {
 };
 Grid grid_of(const Shape& s, int threads = mfcc::kSeqThreads) {
   Grid g;
-  g.v = s.b.ncol % 2 ? 1 : 2;   // values of a row that a thread takes at once
-  g.w.groups = s.b.ncol / g.v;
   g.w.pieces = 1;
   g.w.near = 1;
   // column blocks of at most `wide` groups, equally wide; slots of time: as many as the threads give, at most 64 (each thread
@@ -85,7 +84,16 @@ Grid grid_of(const Shape& s, int threads = mfcc::kSeqThreads) {
     g.w.blocks = (int32_t)blocks_for(s.b.n_seq, g.w.seqs);
     g.w.piece_tiles = (int32_t)std::max<int64_t>((s.longest + g.tile_rows - 1) / g.tile_rows, 1);
   };
-  split(64);   // a wave to a row
+  // values of a row that a thread takes at once: 2, but 1 for narrow rows with many slots of time, every one of which all threads
+  // compose (10000 sequences of 300 rows of 40 bfloat16: 25 slots for 2 values 217 us forward and 547 back, 12 slots for 1 187 and 337)
+  g.v = 2;
+  g.w.groups = s.b.ncol / 2;
+  if (s.b.ncol % 2 == 0) split(64);
+  if (s.b.ncol % 2 || (g.w.cb < kWideBlock && g.w.per > kManySlots)) {
+    g.v = 1;
+    g.w.groups = s.b.ncol;
+    split(64);   // at most a wave to a row
+  }
   const int64_t blocks = (int64_t)g.w.blocks * g.w.column_blocks, tiles = g.w.piece_tiles;
   if (g.w.seqs == 1 && blocks > 0 && blocks < kFewBlocks) {
     const int64_t want = std::min(kTargetBlocks / blocks, tiles / kPieceTiles);   // not one more than the card takes at once
@@ -354,11 +362,19 @@ int mfcc_feature_dropout(const mfcc_layout* layout, int64_t n_seq, int64_t time_
     w.cb = (w.groups + w.column_blocks - 1) / w.column_blocks;
     w.per = 256 / w.cb;
     if (s.rows > most || w.column_blocks > 65535) return fail(MFCC_ERR_UNSUPPORTED, "%s: too many rows or columns per call", who);
-    const dim3 grid(blocks_for((s.rows + 7) / 8, w.per), (unsigned)w.column_blocks);
+    // groups of 8 rows to a thread: as many as leave the card 2048 workgroups (10000 x 300 rows of 39 bfloat16 per sequence: 8 groups
+    // 3.1 TB/s, 1 group 1.2)
+    const int64_t groups = (s.rows + 7) / 8;
+    int runs = mfcc::kDropRuns;
+    while (runs > 1 && groups / (w.per * runs) * w.column_blocks < 2048) runs /= 2;
+    const dim3 grid(blocks_for(groups, w.per * runs), (unsigned)w.column_blocks);
+    auto linear = [&](const mfcc_rows* r) { return s.b.steps == 0 || s.b.n_seq == 1 || r->seq_stride == s.b.steps * r->row_stride; };
+    const bool lin = linear(x) && linear(y), frame = per == MFCC_DROP_FRAME;
     dispatch(rows_dtype, v, true, [&](auto zero, auto vv, auto) {
       using T = decltype(zero);
-      auto k = per == MFCC_DROP_FRAME ? mfcc::dropout_rows_kernel<T, vv(), true> : mfcc::dropout_rows_kernel<T, vv(), false>;
-      hipLaunchKernelGGL(k, grid, dim3(256), 0, st, s.b, w, s.rows, d, rows_of<const T>(x, s), rows_of<T>(y, s));
+      auto k = frame ? (lin ? mfcc::dropout_rows_kernel<T, vv(), true, true> : mfcc::dropout_rows_kernel<T, vv(), true, false>)
+                     : (lin ? mfcc::dropout_rows_kernel<T, vv(), false, true> : mfcc::dropout_rows_kernel<T, vv(), false, false>);
+      hipLaunchKernelGGL(k, grid, dim3(256), 0, st, s.b, w, runs, s.rows, d, rows_of<const T>(x, s), rows_of<T>(y, s));
     });
   }
   HIP_TRY(hipGetLastError());
