@@ -108,7 +108,12 @@ def _out(out, shape, dtype, device):
         raise ValueError(f"out must be a {dtype} device tensor {tuple(shape)} with unit column stride")
     if out.requires_grad:
         raise ValueError("out requires a gradient")
+    _written(out)
     return out
+
+
+# a caller's tensor that a kernel writes counts as changed in place: a graph that saved it refuses its backward pass
+_written = torch.autograd.graph.increment_version
 
 
 def _ptr(t):
@@ -232,8 +237,12 @@ def gated_scan_step(x, gate, state, form="decay", out=None, state_out=None):
     y = _out(out, x.shape, x.dtype, x.device)
     if state_out is None:
         state_out = torch.empty_like(state)
-    elif _check_state(state_out, "state_out", x.shape) is not state and not state_out.is_contiguous():
-        raise ValueError("state_out must be contiguous")
+    else:
+        if _check_state(state_out, "state_out", x.shape) is not state and not state_out.is_contiguous():
+            raise ValueError("state_out must be contiguous")
+        if state_out.requires_grad:
+            raise ValueError("state_out requires a gradient")
+        _written(state_out)
     n, d = x.shape
     with _on(x.device, gate, state, state_out, y):
         capi.check(capi.load().mfcc_gated_scan_step(n, d, _ROWS[x.dtype], _FORMS[form], x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0),
@@ -271,10 +280,14 @@ def running_norm(feats, frame_counts=None, decay=0.995, state=None, eps=1e-5, ce
     y = _out(out, feats.shape, dtype, feats.device)
     if state_out is None:
         state_out = torch.empty(shape, dtype=torch.float32, device=feats.device)
-    elif not _check_state(state_out, "state_out", shape).is_contiguous():
-        raise ValueError("state_out must be contiguous")
-    if state is not None and state_out.data_ptr() == state.data_ptr() and state_out.numel():
-        raise ValueError("state_out must be an array of its own")
+    else:
+        if not _check_state(state_out, "state_out", shape).is_contiguous():
+            raise ValueError("state_out must be contiguous")
+        if state_out.requires_grad:
+            raise ValueError("state_out requires a gradient")
+        if state is not None and state_out.data_ptr() == state.data_ptr() and state_out.numel():
+            raise ValueError("state_out must be an array of its own")
+        _written(state_out)
     if state is not None and not state.is_contiguous():
         state = state.contiguous()
     with _on(feats.device, state, state_out, y):

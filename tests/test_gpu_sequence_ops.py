@@ -827,3 +827,23 @@ def test_padding_is_not_read_and_audio_layouts(M):
     assert torch.equal(M.running_norm(feats, lay)[0], M.running_norm(feats, counts)[0])
     assert torch.equal(M.gated_scan(feats, torch.sigmoid(feats), lay)[0], M.gated_scan(feats, torch.sigmoid(feats), torch.from_numpy(counts))[0])
     assert torch.equal(M.feature_dropout(feats, 0.5, 1, per="sequence", frame_counts=lay), M.feature_dropout(feats, 0.5, 1, per="sequence", frame_counts=counts))
+
+
+@pytest.mark.parametrize("what", ["scan", "step", "step state", "norm", "norm state", "dropout"])
+def test_written_tensors_count_as_changed(M, what):
+    """A tensor that a product saved for its backward pass, then written as out= / state_out=: an error, no wrong gradient."""
+    d = 6
+    x, g, h = (torch.rand(5, d, device="cuda") for _ in range(3))
+    w = torch.ones((1, 1 + 2 * d) if what == "norm state" else (5, d), device="cuda", requires_grad=True)
+    t = torch.rand(w.shape, device="cuda")
+    loss = (w * t).sum()
+    calls = {"scan": lambda t: M.gated_scan(x, g, out=t), "step": lambda t: M.gated_scan_step(x, g, h, out=t),
+             "step state": lambda t: M.gated_scan_step(x, g, h, state_out=t), "norm": lambda t: M.running_norm(x, out=t),
+             "norm state": lambda t: M.running_norm(x, state_out=t), "dropout": lambda t: M.feature_dropout(x, 0.5, 1, out=t)}
+    calls[what](t)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.no_grad(), pytest.raises(ValueError, match="requires a gradient"):
+        calls[what](w)
+    with torch.inference_mode():
+        calls[what](torch.rand(w.shape, device="cuda"))
