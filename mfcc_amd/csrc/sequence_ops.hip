@@ -15,6 +15,8 @@ namespace {
 constexpr int64_t kMaxColumns = 1 << 20;
 constexpr int64_t kMaxSeqs = 1 << 24;
 constexpr int64_t kMaxRows = 1 << 30;  // of one sequence: row numbers inside it are 32-bit
+constexpr double kMaxValues = 1ll << 56;  // counts of values and bytes stay far inside 64 bits
+constexpr int64_t kMaxThreads = UINT32_MAX;  // of one launch, in one direction of its grid: a launch counts threads in 32 bits
 
 // The geometry of a call, checked once: 0 or a negative error code.
 struct Shape {
@@ -30,6 +32,7 @@ int shape_of(const char* who, const mfcc_layout* layout, int64_t n_seq, int64_t 
   out->longest = layout ? (time_steps ? std::min(layout->longest, time_steps) : layout->longest) : time_steps;
   out->rows = time_steps || !layout ? n_seq * time_steps : layout->total_frames;
   if (out->longest > kMaxRows) return fail(MFCC_ERR_UNSUPPORTED, "%s: a sequence of more than 2^30 rows", who);
+  if ((double)out->rows * ncol > kMaxValues) return fail(MFCC_ERR_UNSUPPORTED, "%s: more than 2^56 values", who);
   return MFCC_OK;
 }
 
@@ -109,8 +112,8 @@ Grid grid_of(const Shape& s, int threads = mfcc::kSeqThreads) {
   return g;
 }
 
-int check_grid(const char* who, const Shape& s, const Grid& g, const void* workspace) {
-  if ((s.b.n_seq + 7) * g.w.column_blocks > INT32_MAX)
+int check_grid(const char* who, const Shape& s, const Grid& g, const void* workspace, int threads = mfcc::kSeqThreads) {
+  if (((int64_t)g.w.blocks + 7) / 8 * 8 * g.w.column_blocks > kMaxThreads / threads)
     return fail(MFCC_ERR_UNSUPPORTED, "%s: %lld sequences of %d columns are more than one launch covers", who, (long long)s.b.n_seq, s.b.ncol);
   if (g.w.pieces > 1 && (!workspace || ((uintptr_t)workspace & 15)))
     return fail(MFCC_ERR_INVALID, "%s: this shape needs a 16-byte aligned workspace (mfcc_sequence_workspace)", who);
@@ -250,6 +253,7 @@ int mfcc_gated_scan_step(int64_t n_seq, int32_t ncol, int32_t rows_dtype, int32_
   if (n_seq > 1 && y_ld < ncol) return fail(MFCC_ERR_INVALID, "%s: rows of y overlap", who);
   if (form != MFCC_SCAN_DECAY && form != MFCC_SCAN_SIGMOID) return fail(MFCC_ERR_INVALID, "%s: form=%d", who, form);
   if (n_seq == 0) return MFCC_OK;
+  if (n_seq * ncol > kMaxThreads - 255) return fail(MFCC_ERR_UNSUPPORTED, "%s: too many values per call", who);
   if (!x || !gate || !state_in || !state_out || !y) return fail(MFCC_ERR_INVALID, "%s: null pointer", who);
   auto go = [&](auto zero) {
     using T = decltype(zero);
@@ -283,7 +287,10 @@ int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_ste
   Grid c = grid_of(s);
   if (const int rc = check_grid(who, s, c, workspace)) return rc;
   int threads = mfcc::kSeqThreads;
-  if (c.w.pieces == 1 && (int64_t)c.w.blocks * c.w.column_blocks >= kManyBlocks) c = grid_of(s, threads = mfcc::kSeqThreads / 2);
+  if (c.w.pieces == 1 && (int64_t)c.w.blocks * c.w.column_blocks >= kManyBlocks) {
+    c = grid_of(s, threads = mfcc::kSeqThreads / 2);
+    if (const int rc = check_grid(who, s, c, workspace, threads)) return rc;
+  }
   const size_t size = y_dtype == MFCC_ROWS_F32 ? 4 : 2;
   const bool al = aligned(x, s, c.v, 4) && aligned(y, s, c.v, size);
   c.w.near = near(x, c, s, 4) && near(y, c, s, size);
@@ -347,7 +354,7 @@ int mfcc_feature_dropout(const mfcc_layout* layout, int64_t n_seq, int64_t time_
   };
   if (per == MFCC_DROP_ELEMENT) {
     const int64_t blocks = (s.rows * ncol + 8 * 256 - 1) / (8 * 256);
-    if (blocks > INT32_MAX) return fail(MFCC_ERR_UNSUPPORTED, "%s: too many rows per call", who);
+    if (blocks > kMaxThreads / 256) return fail(MFCC_ERR_UNSUPPORTED, "%s: too many rows per call", who);
     const bool fl = flat(x) && flat(y);
     dispatch(rows_dtype, 1, true, [&](auto zero, auto, auto) {
       using T = decltype(zero);
@@ -367,6 +374,7 @@ int mfcc_feature_dropout(const mfcc_layout* layout, int64_t n_seq, int64_t time_
     const int64_t groups = (s.rows + 7) / 8;
     int runs = mfcc::kDropRuns;
     while (runs > 1 && groups / (w.per * runs) * w.column_blocks < 2048) runs /= 2;
+    if ((groups + w.per * runs - 1) / (w.per * runs) > kMaxThreads / 256) return fail(MFCC_ERR_UNSUPPORTED, "%s: too many rows per call", who);
     const dim3 grid(blocks_for(groups, w.per * runs), (unsigned)w.column_blocks);
     auto linear = [&](const mfcc_rows* r) { return s.b.steps == 0 || s.b.n_seq == 1 || r->seq_stride == s.b.steps * r->row_stride; };
     const bool lin = linear(x) && linear(y), frame = per == MFCC_DROP_FRAME;

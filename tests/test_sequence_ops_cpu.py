@@ -86,3 +86,20 @@ def test_host_tensors_are_refused():
             mfcc_amd.running_norm_state(bad, 1.0)
     with pytest.raises(ValueError):
         mfcc_amd.running_norm_state(sums, -1.0)
+
+
+@pytest.mark.parametrize("call", [
+    # more threads than one launch counts (2^32 - 1): workgroups are sequences x column blocks
+    # (2^20 columns: 8192 blocks of 64 pairs; 100 rows take a workgroup of 512 threads to themselves: 1024 x 8192 x 512 = 2^32)
+    lambda l: scan(l, n=1024, steps=100, ncol=1 << 20, y=rows(100 << 20, 1 << 20)),
+    lambda l: norm(l, n=1 << 24, steps=600, ncol=64, x=rows(38400, 64), y=rows(38400, 64)),
+    lambda l: drop(l, n=1 << 24, steps=300, ncol=8, x=rows(2400, 8), y=rows(2400, 8)),
+    lambda l: step(l, n=1 << 24, ncol=256, x_ld=256, y_ld=256),
+    # products that would pass 63 bits
+    lambda l: scan(l, n=1 << 24, steps=1 << 30, ncol=1 << 20, y=rows(1 << 50, 1 << 20)),
+    lambda l: drop(l, n=1 << 24, steps=1 << 30, ncol=1 << 20, y=rows(1 << 50, 1 << 20)),
+    lambda l: l.mfcc_gated_scan_checkpoints(None, 1 << 24, 1 << 30, 1 << 20, 0),
+    lambda l: l.mfcc_sequence_workspace(None, 1 << 24, 1 << 30, 1 << 20, 0)])
+def test_what_one_launch_does_not_cover_is_refused(lib, call):
+    assert call(lib) == capi.ERR_UNSUPPORTED
+    assert lib.mfcc_last_error()
