@@ -281,7 +281,8 @@ int mfcc_pad_batch(const mfcc_layout* layout, const float* feats, int64_t feats_
  * seq_stride at data + (frame_offset[u] + t) * row_stride + c when time_steps = 0.  Inputs may have any
  * strides >= 0 (row_stride 0: one row for all); rows of outputs must not overlap.  Rows behind the end of a
  * padded sequence are never read; outputs get 0 there.  Sequences may be empty.  At most 2^30 rows per
- * sequence, 2^24 sequences.  Rows are float32, bfloat16 or float16; states are float32 and the arithmetic is float32. */
+ * sequence, 2^24 sequences, 2^20 columns; MFCC_ERR_UNSUPPORTED for what would count more than 2^32 threads in a launch.
+ * Rows are float32, bfloat16 or float16; states are float32 and the arithmetic is float32. */
 #define MFCC_ROWS_F32 0
 #define MFCC_ROWS_BF16 1
 #define MFCC_ROWS_F16 2

@@ -989,21 +989,21 @@ __global__ void __launch_bounds__(256) dropout_element_kernel(const Batch b, int
     if (i < k) y.p[to[i]] = gone >> i & 1 ? (T)0.0f : (T)(v[i] * d.scale);
 }
 
-// per = frame or sequence: a thread takes V columns of `runs` groups of 8 rows, loading a group at a time.  A block decides 8 rows:
-// it is made once for the workgroup (LDS); or 8 columns for as long as the sequence lasts: a thread makes it again where the sequence
-// changes.  More groups a thread share the search for the first row's sequence and the blocks, fewer fill the card.
+// per = frame or sequence: a thread takes V columns of `runs` groups of 8 rows, loading a group at a time.  Per frame (runs is 1) a
+// block decides the 8 rows of a slot and is made once for the workgroup (LDS); per sequence it decides 8 columns for as long as the
+// sequence lasts, and a thread makes it again where the sequence changes: more groups a thread share the search for the first row's
+// sequence and the blocks, fewer fill the card.
 // LINEAR: row number times row stride is the address, padded batches included.
-// Bound: HBM, read once and written once: 256 x 1024 rows of 512 float16 5.0 to 5.2 TB/s; 39 columns of bfloat16 3.1 to 3.5, two
+// Bound: HBM, read once and written once: 256 x 1024 rows of 512 float16 5.8 and 5.0 TB/s; 39 columns of bfloat16 4.0 and 3.1, two
 // bytes a lane.  64 utterances of 39 floats: 5 us, the launch and the search.
-constexpr int kDropRuns = 8;
 template <typename T, int V, bool FRAME, bool LINEAR>
 __global__ void __launch_bounds__(256) dropout_rows_kernel(const Batch b, const Split w, int runs, int64_t n_rows, const Dropout d,
                                                            const Rows<const T> x, const Rows<T> y) {
-  __shared__ uint32_t rows_gone[256 * kDropRuns];
+  __shared__ uint32_t rows_gone[256];
   const int slot = threadIdx.x / w.cb, group = blockIdx.y * w.cb + (threadIdx.x - slot * w.cb);
   const int64_t first = (int64_t)blockIdx.x * w.per * runs, step = (int64_t)d.at();   // the first group of 8 rows of the workgroup
   if (FRAME) {
-    for (int i = threadIdx.x; i < w.per * runs; i += 256) rows_gone[i] = philox_dropped((uint64_t)(first + i), step, d.seed, d.threshold);
+    if (threadIdx.x < w.per) rows_gone[threadIdx.x] = philox_dropped((uint64_t)(first + threadIdx.x), step, d.seed, d.threshold);
     __syncthreads();
   }
   const int64_t r0 = (first + slot * runs) * 8;
@@ -1034,7 +1034,7 @@ __global__ void __launch_bounds__(256) dropout_rows_kernel(const Batch b, const 
 #pragma unroll
       for (int i = 0; i < 8; ++i) load_pack<true>(v[i], x.p + (r + min(i, k - 1)) * x.rs + col);
     }
-    if (FRAME) gone = rows_gone[slot * runs + g];
+    if (FRAME) gone = rows_gone[slot];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if (i >= k) break;

@@ -369,15 +369,17 @@ int mfcc_feature_dropout(const mfcc_layout* layout, int64_t n_seq, int64_t time_
     w.cb = (w.groups + w.column_blocks - 1) / w.column_blocks;
     w.per = 256 / w.cb;
     if (s.rows > most || w.column_blocks > 65535) return fail(MFCC_ERR_UNSUPPORTED, "%s: too many rows or columns per call", who);
-    // groups of 8 rows to a thread: as many as leave the card 2048 workgroups (10000 x 300 rows of 39 bfloat16 per sequence: 8 groups
-    // 3.1 TB/s, 1 group 1.2)
+    // groups of 8 rows to a thread: per frame 1; per sequence as many as leave the card 2048 workgroups, but 1 where the 8 rows of a few
+    // columns are far from the next thread's (10000 x 300 rows of 39 bfloat16: per frame 1 group 4.0 TB/s, 8 groups 3.5; per sequence
+    // 1.6 and 3.1; 20000 x 500 rows of 4 floats per sequence 3.0 and 2.7, of 8 floats 3.8 and 3.5, 10000 x 300 of 13 2.5 and 3.0)
     const int64_t groups = (s.rows + 7) / 8;
-    int runs = mfcc::kDropRuns;
+    const bool frame = per == MFCC_DROP_FRAME;
+    int runs = frame || w.cb < 8 ? 1 : 8;
     while (runs > 1 && groups / (w.per * runs) * w.column_blocks < 2048) runs /= 2;
     if ((groups + w.per * runs - 1) / (w.per * runs) > kMaxThreads / 256) return fail(MFCC_ERR_UNSUPPORTED, "%s: too many rows per call", who);
     const dim3 grid(blocks_for(groups, w.per * runs), (unsigned)w.column_blocks);
     auto linear = [&](const mfcc_rows* r) { return s.b.steps == 0 || s.b.n_seq == 1 || r->seq_stride == s.b.steps * r->row_stride; };
-    const bool lin = linear(x) && linear(y), frame = per == MFCC_DROP_FRAME;
+    const bool lin = linear(x) && linear(y);
     dispatch(rows_dtype, v, true, [&](auto zero, auto vv, auto) {
       using T = decltype(zero);
       auto k = frame ? (lin ? mfcc::dropout_rows_kernel<T, vv(), true, true> : mfcc::dropout_rows_kernel<T, vv(), true, false>)
