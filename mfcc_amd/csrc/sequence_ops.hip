@@ -66,7 +66,7 @@ constexpr int kWideBlock = 40, kManySlots = 12;
 // How workgroups divide sequences, columns and time.  It depends on the shape of the batch alone, so that the backward
 // pass finds its checkpoints whatever the alignment of its arrays.
 struct Grid {
-  int v, tile_rows;
+  int v, tile_rows, threads;   // threads: of a workgroup, the waves that hold all its slots
   mfcc::Split w;
   dim3 blocks;
 };
@@ -109,11 +109,13 @@ Grid grid_of(const Shape& s, int threads = mfcc::kSeqThreads) {
     }
   }
   g.blocks = dim3((unsigned)((g.w.blocks + 7) / 8 * 8 * g.w.column_blocks));
+  // 64 slots of fewer than 8 columns are not 8 waves (20000 sequences of 2000 floats: scan 218 us in one wave, 500 in eight)
+  g.threads = std::min(threads, (g.w.seqs * g.w.per * g.w.cb + 63) / 64 * 64); 
   return g;
 }
 
-int check_grid(const char* who, const Shape& s, const Grid& g, const void* workspace, int threads = mfcc::kSeqThreads) {
-  if (((int64_t)g.w.blocks + 7) / 8 * 8 * g.w.column_blocks > kMaxThreads / threads)
+int check_grid(const char* who, const Shape& s, const Grid& g, const void* workspace) {
+  if (((int64_t)g.w.blocks + 7) / 8 * 8 * g.w.column_blocks > kMaxThreads / g.threads)
     return fail(MFCC_ERR_UNSUPPORTED, "%s: %lld sequences of %d columns are more than one launch covers", who, (long long)s.b.n_seq, s.b.ncol);
   if (g.w.pieces > 1 && (!workspace || ((uintptr_t)workspace & 15)))
     return fail(MFCC_ERR_INVALID, "%s: this shape needs a 16-byte aligned workspace (mfcc_sequence_workspace)", who);
@@ -195,11 +197,10 @@ int mfcc_gated_scan(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps
     if (c.w.pieces > 1) {
       auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_pieces_kernel<T, v(), al(), true, false>
                                          : mfcc::gated_scan_pieces_kernel<T, v(), al(), false, false>;
-      hipLaunchKernelGGL(k, c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const T>(x, s),
-                         rows_of<const T>(gate, s), q);
+      hipLaunchKernelGGL(k, c.blocks, dim3(c.threads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const T>(x, s), rows_of<const T>(gate, s), q);
     }
     auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_kernel<T, v(), al(), true> : mfcc::gated_scan_kernel<T, v(), al(), false>;
-    hipLaunchKernelGGL(k, c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const T>(x, s), rows_of<const T>(gate, s),
+    hipLaunchKernelGGL(k, c.blocks, dim3(c.threads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const T>(x, s), rows_of<const T>(gate, s),
                        rows_of<T>(y, s), q);
   });
   HIP_TRY(hipGetLastError());
@@ -235,11 +236,11 @@ int mfcc_gated_scan_backward(const mfcc_layout* layout, int64_t n_seq, int64_t t
     if (c.w.pieces > 1) {
       auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_pieces_kernel<T, v(), al(), true, true>
                                          : mfcc::gated_scan_pieces_kernel<T, v(), al(), false, true>;
-      hipLaunchKernelGGL(k, c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const T>(grad_y, s),
+      hipLaunchKernelGGL(k, c.blocks, dim3(c.threads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const T>(grad_y, s),
                          rows_of<const T>(gate, s), q);
     }
     auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_backward_kernel<T, v(), al(), true> : mfcc::gated_scan_backward_kernel<T, v(), al(), false>;
-    hipLaunchKernelGGL(k, c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const T>(x, s), rows_of<const T>(gate, s),
+    hipLaunchKernelGGL(k, c.blocks, dim3(c.threads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const T>(x, s), rows_of<const T>(gate, s),
                        rows_of<const T>(grad_y, s), rows_of<T>(grad_x, s), rows_of<T>(grad_gate, s), q);
   });
   HIP_TRY(hipGetLastError());
@@ -286,10 +287,9 @@ int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_ste
   if (s.b.n_seq == 0) return MFCC_OK;
   Grid c = grid_of(s);
   if (const int rc = check_grid(who, s, c, workspace)) return rc;
-  int threads = mfcc::kSeqThreads;
   if (c.w.pieces == 1 && (int64_t)c.w.blocks * c.w.column_blocks >= kManyBlocks) {
-    c = grid_of(s, threads = mfcc::kSeqThreads / 2);
-    if (const int rc = check_grid(who, s, c, workspace, threads)) return rc;
+    c = grid_of(s, mfcc::kSeqThreads / 2);
+    if (const int rc = check_grid(who, s, c, workspace)) return rc;
   }
   const size_t size = y_dtype == MFCC_ROWS_F32 ? 4 : 2;
   const bool al = aligned(x, s, c.v, 4) && aligned(y, s, c.v, size);
@@ -321,11 +321,10 @@ int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_ste
   dispatch(y_dtype, c.v, al, [&](auto zero, auto v, auto al) {
     using T = decltype(zero);
     if (c.w.pieces > 1)
-      hipLaunchKernelGGL((mfcc::running_norm_pieces_kernel<v(), al()>), c.blocks, dim3(mfcc::kSeqThreads), 0, (hipStream_t)stream, s.b, c.w,
-                         rows_of<const float>(x, s), a);
+      hipLaunchKernelGGL((mfcc::running_norm_pieces_kernel<v(), al()>), c.blocks, dim3(c.threads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const float>(x, s), a);
     const int slots = c.w.seqs * c.w.per;
     const size_t shared = 2 * slots * ((1 + mfcc::kSlotRows / 4) * sizeof(float4) + v() * c.w.cb * sizeof(float2));
-    hipLaunchKernelGGL((mfcc::running_norm_kernel<T, v(), al()>), c.blocks, dim3(threads), shared, (hipStream_t)stream, s.b, c.w,
+    hipLaunchKernelGGL((mfcc::running_norm_kernel<T, v(), al()>), c.blocks, dim3(c.threads), shared, (hipStream_t)stream, s.b, c.w,
                        rows_of<const float>(x, s), rows_of<T>(y, s), a);
   });
   HIP_TRY(hipGetLastError());
