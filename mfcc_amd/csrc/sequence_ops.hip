@@ -110,7 +110,7 @@ Grid grid_of(const Shape& s, int threads = mfcc::kSeqThreads) {
   }
   g.blocks = dim3((unsigned)((g.w.blocks + 7) / 8 * 8 * g.w.column_blocks));
   // 64 slots of fewer than 8 columns are not 8 waves (20000 sequences of 2000 floats: scan 218 us in one wave, 500 in eight)
-  g.threads = std::min(threads, (g.w.seqs * g.w.per * g.w.cb + 63) / 64 * 64); 
+  g.threads = std::min(threads, (g.w.seqs * g.w.per * g.w.cb + 63) / 64 * 64);
   return g;
 }
 
