@@ -25,10 +25,15 @@ $(LIB): build/mfcc_amd.o $(SEQO)
 	@mkdir -p $(dir $@)
 	$(HIPCC) --offload-arch=$(ARCH) -fPIC -shared -o $@ $^
 
-host_sim: tests/host_sim/fft_sim
+host_sim: tests/host_sim/fft_sim tests/host_sim/libsequence_sim.so
 
 tests/host_sim/fft_sim: tests/host_sim/fft_sim.cpp mfcc_amd/csrc/fft_lane.h mfcc_amd/csrc/tables.h
 	g++ -O2 -std=c++17 -I mfcc_amd/csrc -o $@ $<
+
+# the operators along time as host code (clang for its 16-bit types), for tests/test_sequence_kernels_cpu.py
+HOSTCXX ?= /opt/rocm/llvm/bin/clang++
+tests/host_sim/libsequence_sim.so: tests/host_sim/sequence_sim.cpp tests/host_sim/device/hip/hip_runtime.h $(SEQ) mfcc_amd/csrc/sequence_kernels.h mfcc_amd/csrc/abi.h include/mfcc_amd.h
+	$(HOSTCXX) -x c++ -O1 -std=c++17 -fPIC -shared -ffp-contract=off -Wall -Wno-unused-function -I tests/host_sim/device -o $@ $<
 
 # experimental builds for A/B timing: make variant NAME=noslp EXTRA="-fno-slp-vectorize"
 variant: $(SRC) $(HDRS) $(SEQO)
@@ -49,6 +54,6 @@ asm: $(SRC) $(HDRS)
 	$(HIPCC) --offload-arch=$(ARCH) -O3 -std=c++17 -fno-signed-zeros -fno-slp-vectorize $(EXTRA) -S --cuda-device-only -o build/mfcc_amd.s $(SRC) -Rpass-analysis=kernel-resource-usage 2> build/resource_usage.txt
 
 clean:
-	rm -rf mfcc_amd/lib build tests/host_sim/fft_sim
+	rm -rf mfcc_amd/lib build tests/host_sim/fft_sim tests/host_sim/libsequence_sim.so
 
 .PHONY: all host_sim asm clean variant split

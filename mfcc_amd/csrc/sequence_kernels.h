@@ -100,6 +100,7 @@ struct Seat {
   int64_t u;           // sequence
   Span s;
   int n, sub, slot, cg, col;
+  int wide;            // column groups that the workgroup has: the last block of a row may have fewer than the others
   int piece, tile, tiles, full;  // the tiles [tile, tiles) of the sequence, those below `full` without a missing row
   bool on;             // there is such a sequence
   bool there;          // the workgroup has something to do
@@ -116,9 +117,9 @@ __device__ inline Seat seat_of(const Batch& b, const Split& w) {
   t.piece = at - block * w.pieces;
   t.slot = threadIdx.x / w.cb;
   t.cg = (int)threadIdx.x - t.slot * w.cb;
-  const int groups = w.groups - column_block * w.cb;
-  t.own = t.slot < w.seqs * w.per && t.cg < groups;
-  t.cg = min(t.cg, groups - 1);
+  t.wide = min(w.groups - column_block * w.cb, w.cb);
+  t.own = t.slot < w.seqs * w.per && t.cg < t.wide;
+  t.cg = min(t.cg, t.wide - 1);
   if (t.slot >= w.seqs * w.per) t.slot = 0;
   t.col = (column_block * w.cb + t.cg) * V;
   const int tile_rows = w.per * kSlotRows;
@@ -759,9 +760,9 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batc
 #pragma unroll
     for (int v = 0; v < V; ++v) base[v] = (float)mean[v], off[v] = (float)(mean[v] - base[v]);
     float4* const inv = inverses + (turn * slots + t.slot) * (R / 4);
-    // 1 / w of the rows: the first column groups take one row each
+    // 1 / w of the rows: the column groups that there are take one row each, and further ones where they are fewer than the rows
     if (t.cg < R) ((float*)inv)[t.cg] = __builtin_amdgcn_rcpf(fmaf(own_decayed, ws, own_grown));
-    for (int r = t.cg + w.cb; r < R; r += w.cb) ((float*)inv)[r] = __builtin_amdgcn_rcpf(fmaf(a.decayed[r], ws, a.grown[r]));   // few columns
+    for (int r = t.cg + t.wide; r < R; r += t.wide) ((float*)inv)[r] = __builtin_amdgcn_rcpf(fmaf(a.decayed[r], ws, a.grown[r]));
     if (w.per > 1) {
 #pragma unroll
       for (int v = 0; v < V; ++v) m[v] = 0.0f, q[v] = 0.0f;
