@@ -8,12 +8,14 @@ with frame counts (``MFCC.forward``), or a padded ``[B, T, D]`` batch with lengt
 'post' padding).  ``frame_counts`` is a sequence of counts, a :class:`~mfcc_amd.Layout` (keep one for
 repeated batch shapes; required while a stream is being captured) or None: all rows are one sequence
 (2-D) or every sequence is full (3-D).  Lengths beyond T count as T, as ``pad_sequences`` reports
-them.  Rows behind the end of a padded sequence are not read; outputs hold 0 there.
+them.  Rows behind the end of a padded sequence are not read; outputs hold 0 there.  Derivatives are those of
+backward passes: tensors that carry a forward-mode tangent are refused.
 """
 from __future__ import annotations
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _capi as capi
@@ -137,6 +139,13 @@ def _sizes(batch, code):
 _plain_sizes = {}
 
 
+def _no_tangent(*tensors):
+    """Refuses dual tensors of forward-mode differentiation: they do not require a gradient, so their derivative would be dropped unseen."""
+    if forward_ad._current_level >= 0 and not torch.is_inference_mode_enabled():
+        if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise ValueError("no forward-mode derivative: a tensor carries a tangent")
+
+
 def _no_grad(*tensors):
     return not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
 
@@ -206,6 +215,7 @@ def gated_scan(x, gate, frame_counts=None, h0=None, form="decay", reverse=False,
     ``out`` takes y when no gradient is asked for; it may be ``x``."""
     _check(x, "x")
     _check(gate, "gate", like=x)
+    _no_tangent(x, gate, h0, out)
     if form not in _FORMS:
         raise ValueError("form must be 'decay' or 'sigmoid'")
     batch = _Batch(x, frame_counts)
@@ -229,6 +239,7 @@ def gated_scan_step(x, gate, state, form="decay", out=None, state_out=None):
         raise ValueError("x must be [n_seq, D]")
     if form not in _FORMS:
         raise ValueError("form must be 'decay' or 'sigmoid'")
+    _no_tangent(x, gate, state, out, state_out)
     if not _no_grad(x, gate, state):
         raise ValueError("gated_scan_step has no gradient: call it under torch.no_grad(), or gated_scan with one row a sequence")
     _check_state(state, "state", x.shape)
@@ -267,6 +278,7 @@ def running_norm(feats, frame_counts=None, decay=0.995, state=None, eps=1e-5, ce
     or float16; ``out`` may be ``feats`` when that is float32; ``state_out`` is an array of its own.  Feature rows
     have no gradient here: an input that requires one is refused."""
     _check(feats, "feats", dtypes=(torch.float32,))
+    _no_tangent(feats, state, out, state_out)
     if not _no_grad(feats, state):
         raise ValueError("running_norm has no gradient")
     batch = _Batch(feats, frame_counts)
@@ -354,6 +366,7 @@ def feature_dropout(feats, p, seed, step=0, per="element", frame_counts=None, ou
     [rows, D] or [B, T, D]; all rows of a padded batch are processed.  ``out`` takes the result when no gradient is
     asked for; it may be ``feats``."""
     _check(feats, "feats")
+    _no_tangent(feats, out)
     if per not in _PER:
         raise ValueError("per must be 'element', 'frame' or 'sequence'")
     if not 0.0 <= p <= 1.0:

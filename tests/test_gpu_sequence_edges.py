@@ -24,3 +24,22 @@ def test_norm_last_column_block(M, counts, d):
 def test_scan_last_column_block(M, counts, d):
     check_scan(M, counts, d, torch.float32, "sigmoid", seed=d)
     check_scan(M, counts, d, torch.bfloat16, "decay", reverse=True, seed=d)
+
+
+def test_forward_mode_is_refused(M):
+    """Dual tensors do not require a gradient; every call refuses them instead of returning a value without its tangent."""
+    x, g, h = (torch.rand(5, 6, device="cuda") for _ in range(3))
+    st = torch.rand(1, 13, device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        def dual(t):
+            return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+        calls = [lambda: M.gated_scan(dual(x), g), lambda: M.gated_scan(x, dual(g)), lambda: M.gated_scan(x, g, h0=dual(h[:1])),
+                 lambda: M.gated_scan(x.clone().requires_grad_(True), dual(g)), lambda: M.gated_scan(x, g, out=dual(h.clone())),
+                 lambda: M.gated_scan_step(x, g, dual(h)), lambda: M.gated_scan_step(dual(x), g, h), lambda: M.gated_scan_step(x, g, h, state_out=dual(h)),
+                 lambda: M.running_norm(dual(x)), lambda: M.running_norm(x, state=dual(st)), lambda: M.running_norm(x, out=dual(h.clone())),
+                 lambda: M.feature_dropout(dual(x), 0.5, 1), lambda: M.feature_dropout(x, 0.5, 1, out=dual(h.clone()))]
+        for call in calls:
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(ValueError, match="tangent"):
+                    call()
+        assert torch.equal(M.gated_scan(x, g)[0], M.gated_scan(x, g)[0])    # tensors without one go on as ever
