@@ -279,7 +279,9 @@ int mfcc_pad_batch(const mfcc_layout* layout, const float* feats, int64_t feats_
  * (n_seq is ignored with a layout), and every array of rows by an mfcc_rows: element (sequence u, row t,
  * column c) sits at data + u * seq_stride + t * row_stride + c, strides in elements, without a
  * seq_stride at data + (frame_offset[u] + t) * row_stride + c when time_steps = 0.  Inputs may have any
- * strides >= 0 (row_stride 0: one row for all); rows of outputs must not overlap.  Rows behind the end of a
+ * strides >= 0 (row_stride 0: one row for all); rows of outputs must not overlap.  What a call writes must lie apart
+ * from all its other arrays, but where "may be" says that it may be the same one (same address, same strides); a call
+ * checks that from spans and strides and refuses what overlaps (views whose rows or sequences interleave are fine).  Rows behind the end of a
  * padded sequence are never read; outputs get 0 there.  Sequences may be empty.  At most 2^30 rows per
  * sequence, 2^24 sequences, 2^20 columns; MFCC_ERR_UNSUPPORTED for what would count more than 2^32 threads in a launch.
  * Rows are float32, bfloat16 or float16; states are float32 and the arithmetic is float32. */
@@ -299,7 +301,7 @@ typedef struct mfcc_rows {
  * last row, h0 for an empty sequence.  reverse = 1: t runs from the last row of a sequence to its first.
  * checkpoints: NULL, or mfcc_gated_scan_checkpoints() floats that receive states for the backward pass.
  * workspace: mfcc_sequence_workspace() bytes of device memory, 16-byte aligned, used by this call only (may be NULL
- * where that is 0).  y may be x (same strides). */
+ * where that is 0).  y may be x or gate. */
 #define MFCC_SCAN_DECAY 0
 #define MFCC_SCAN_SIGMOID 1
 int64_t mfcc_gated_scan_checkpoints(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype);
@@ -308,15 +310,15 @@ int mfcc_gated_scan(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps
                     int32_t reverse, const mfcc_rows* x, const mfcc_rows* gate, const float* h0, const mfcc_rows* y, float* last,
                     float* checkpoints, void* workspace, void* stream);
 /* Gradients of mfcc_gated_scan: from grad_y (rows; NULL = 0) and grad_last (float32 [n_seq, ncol]; NULL = 0) to grad_x,
- * grad_gate (rows) and grad_h0 (float32 [n_seq, ncol]; may be NULL), which overlap none of the inputs.  x, gate, h0, checkpoints and the geometry are the
- * forward call's.  The states are computed again in float32 from the checkpoints, so grad_gate does not suffer from
+ * grad_gate (rows) and grad_h0 (float32 [n_seq, ncol]; may be NULL).  x, gate, h0, checkpoints and the geometry are the forward call's.  The states are computed again in float32 from the checkpoints, so grad_gate does not suffer from
  * the rounding of y. */
 int mfcc_gated_scan_backward(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype, int32_t form,
                              int32_t reverse, const mfcc_rows* x, const mfcc_rows* gate, const float* checkpoints,
                              const mfcc_rows* grad_y, const float* grad_last, const mfcc_rows* grad_x, const mfcc_rows* grad_gate,
                              float* grad_h0, void* workspace, void* stream);
 /* One step of the same recurrence for n_seq live sequences: x, gate, y rows [n_seq, ncol] with row strides in
- * elements, state_in / state_out float32 [n_seq, ncol] contiguous, which may be the same array. */
+ * elements, state_in / state_out float32 [n_seq, ncol] contiguous, which may be the same array; y may be x or gate, and
+ * any array a state of its type and strides. */
 int mfcc_gated_scan_step(int64_t n_seq, int32_t ncol, int32_t rows_dtype, int32_t form, const void* x, int64_t x_ld, const void* gate,
                          int64_t gate_ld, const float* state_in, float* state_out, void* y, int64_t y_ld, void* stream);
 
@@ -327,7 +329,7 @@ int mfcc_gated_scan_step(int64_t n_seq, int32_t ncol, int32_t rows_dtype, int32_
  * 0 < decay <= 1 (1: cumulative statistics; exact up to 2^24 rows), eps >= 0.  The streaming counterpart of the
  * corpus constants (x + mm) .* vv (anal_recog_nn_liste.m:180) and of the per-utterance (x - mean) / std
  * (inference_ctc_eri_05.py:291), which need the whole corpus or utterance.  x is float32; y has y_dtype and may be x
- * when that is float32 (same strides).  state_out (may be NULL): the state
+ * when that is float32.  state_out (may be NULL): the state
  * behind the last row, in an array of its own. */
 int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, double decay, double eps,
                       int32_t center_only, const mfcc_rows* x, const float* state_in, const mfcc_rows* y, int32_t y_dtype,
@@ -343,7 +345,7 @@ int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_ste
  *   MFCC_DROP_SEQUENCE  u * ceil(ncol / 8) * 8 + c          a column is dropped for a whole sequence
  * Applied to a gradient with the same arguments it is the backward pass.  step_device: NULL, or a device int64 that is
  * read instead of `step` when the kernel runs (for a captured graph whose replays draw new masks).  All rows of a padded
- * batch are processed.  layout may be NULL with time_steps = rows, n_seq = 1.  y may be x (same strides). */
+ * batch are processed.  layout may be NULL with time_steps = rows, n_seq = 1.  y may be x. */
 #define MFCC_DROP_ELEMENT 0
 #define MFCC_DROP_FRAME 1
 #define MFCC_DROP_SEQUENCE 2

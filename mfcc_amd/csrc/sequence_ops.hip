@@ -1,6 +1,8 @@
 // C entry points of the operators along time (see "operators along time over feature rows" in include/mfcc_amd.h).
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
+#include <numeric>
 #include <type_traits>
 
 #include "abi.h"
@@ -16,6 +18,7 @@ constexpr int64_t kMaxColumns = 1 << 20;
 constexpr int64_t kMaxSeqs = 1 << 24;
 constexpr int64_t kMaxRows = 1 << 30;  // of one sequence: row numbers inside it are 32-bit
 constexpr double kMaxValues = 1ll << 56;  // counts of values and bytes stay far inside 64 bits
+constexpr int64_t kMaxStride = 1ll << 56;
 constexpr int64_t kMaxThreads = UINT32_MAX;  // of one launch, in one direction of its grid: a launch counts threads in 32 bits
 
 // The geometry of a call, checked once: 0 or a negative error code.
@@ -39,6 +42,7 @@ int shape_of(const char* who, const mfcc_layout* layout, int64_t n_seq, int64_t 
 int check_rows(const char* who, const char* name, const mfcc_rows* r, const Shape& s, bool output) {
   if (!r || (!r->data && s.rows > 0)) return fail(MFCC_ERR_INVALID, "%s: %s is null", who, name);
   if (r->row_stride < 0 || r->seq_stride < 0) return fail(MFCC_ERR_INVALID, "%s: negative stride of %s", who, name);
+  if (r->row_stride > kMaxStride || r->seq_stride > kMaxStride) return fail(MFCC_ERR_INVALID, "%s: a stride of %s passes 2^56", who, name);
   if (output && s.rows > 1) {
     // rows of outputs do not overlap: one row after the other inside a sequence and sequence after sequence, or
     // time-major (all sequences' row t, then row t + 1)
@@ -114,6 +118,13 @@ Grid grid_of(const Shape& s, int threads = mfcc::kSeqThreads) {
   return g;
 }
 
+// Floats of the checkpoints, bytes of the workspace.
+int64_t checkpoints_of(const Shape& s, const Grid& g) {
+  const int64_t k = g.tile_rows, t = s.b.steps;
+  return (t || !s.b.off ? s.b.n_seq * ((t + k - 1) / k) : s.rows / k + s.b.n_seq) * s.b.ncol;
+}
+int64_t workspace_of(const Shape& s, const Grid& g) { return g.w.pieces > 1 ? s.b.n_seq * g.w.pieces * s.b.ncol * (int64_t)sizeof(float2) : 0; }
+
 int check_grid(const char* who, const Shape& s, const Grid& g, const void* workspace) {
   if (((int64_t)g.w.blocks + 7) / 8 * 8 * g.w.column_blocks > kMaxThreads / g.threads)
     return fail(MFCC_ERR_UNSUPPORTED, "%s: %lld sequences of %d columns are more than one launch covers", who, (long long)s.b.n_seq, s.b.ncol);
@@ -152,6 +163,50 @@ Rows<T> rows_of(const mfcc_rows* r, const Shape& s) {
   return r && s.rows > 0 ? Rows<T>{(T*)r->data, r->seq_stride, r->row_stride} : Rows<T>{nullptr, 0, 0};
 }
 
+// The bytes that a call reads or writes through one argument: `seqs` blocks of `rows` rows of `width` bytes.
+struct Bytes {
+  const char* name;
+  const char* p;
+  int64_t width;
+  int64_t row, seq;   // strides, 0 where there is but one
+  int64_t rows, seqs;
+};
+Bytes bytes_of(const char* name, const mfcc_rows* r, const Shape& s, size_t size) {
+  Bytes a{name, r && s.rows > 0 ? (const char*)r->data : nullptr, s.b.ncol * (int64_t)size, 0, 0, s.b.steps ? s.b.steps : s.rows, s.b.steps ? s.b.n_seq : 1};
+  if (!a.p) return a;
+  if (a.rows > 1) a.row = r->row_stride * (int64_t)size;
+  if (a.seqs > 1) a.seq = r->seq_stride * (int64_t)size;
+  return a;
+}
+Bytes bytes_of(const char* name, const void* p, int64_t bytes) { return Bytes{name, bytes > 0 ? (const char*)p : nullptr, bytes, 0, 0, 1, 1}; }
+
+// No byte of a is one of b, as far as spans and strides tell: the whole spans, what lies between sequences, what lies between rows.
+bool apart(const Bytes& a, const Bytes& b) {
+  typedef __int128 wide;
+  if (!a.p || !b.p) return true;
+  const wide d = (wide)(intptr_t)b.p - (intptr_t)a.p;
+  auto seq_span = [](const Bytes& x) { return (wide)(x.rows - 1) * x.row + x.width; };
+  auto row_span = [](const Bytes& x) { return (wide)(x.seqs - 1) * x.seq + x.width; };
+  if (d >= seq_span(a) + (wide)(a.seqs - 1) * a.seq || -d >= seq_span(b) + (wide)(b.seqs - 1) * b.seq) return true;
+  auto between = [&](int64_t period, wide wa, wide wb) {   // both repeat with this period
+    if (period <= 0) return false;
+    const wide at = (d % period + period) % period;
+    return at >= wa && period - at >= wb;
+  };
+  const int64_t seqs = std::gcd(a.seq, b.seq), rows = std::gcd(a.row, b.row);
+  return between(seqs, seq_span(a), seq_span(b)) || between(rows, row_span(a), row_span(b)) || between(std::gcd(seqs, rows), a.width, b.width);
+}
+bool same(const Bytes& a, const Bytes& b) { return a.p == b.p && a.width == b.width && a.row == b.row && a.seq == b.seq; }
+
+// Threads read and write in no order between workgroups: what a call writes lies apart from everything else, but for the arrays that it
+// may work on in place.
+int check_apart(const char* who, const Bytes& out, std::initializer_list<Bytes> others, bool in_place = false) {
+  for (const Bytes& o : others)
+    if (!apart(out, o) && !(in_place && same(out, o)))
+      return fail(MFCC_ERR_INVALID, in_place ? "%s: %s overlaps %s without being the same rows" : "%s: %s overlaps %s", who, out.name, o.name);
+  return MFCC_OK;
+}
+
 int bad_dtype(const char* who, int32_t dtype) { return fail(MFCC_ERR_INVALID, "%s: rows type %d", who, dtype); }
 
 }  // namespace
@@ -162,16 +217,14 @@ int64_t mfcc_gated_scan_checkpoints(const mfcc_layout* layout, int64_t n_seq, in
   Shape s;
   if (const int rc = shape_of("mfcc_gated_scan_checkpoints", layout, n_seq, time_steps, ncol, 0, &s)) return rc;
   if (rows_dtype < 0 || rows_dtype > MFCC_ROWS_F16) return bad_dtype("mfcc_gated_scan_checkpoints", rows_dtype);
-  const int64_t k = grid_of(s).tile_rows;
-  return (time_steps || !layout ? s.b.n_seq * ((time_steps + k - 1) / k) : s.rows / k + s.b.n_seq) * ncol;
+  return checkpoints_of(s, grid_of(s));
 }
 
 int64_t mfcc_sequence_workspace(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype) {
   Shape s;
   if (const int rc = shape_of("mfcc_sequence_workspace", layout, n_seq, time_steps, ncol, 0, &s)) return rc;
   if (rows_dtype < 0 || rows_dtype > MFCC_ROWS_F16) return bad_dtype("mfcc_sequence_workspace", rows_dtype);
-  const Grid g = grid_of(s);
-  return g.w.pieces > 1 ? s.b.n_seq * g.w.pieces * ncol * (int64_t)sizeof(float2) : 0;
+  return workspace_of(s, grid_of(s));
 }
 
 int mfcc_gated_scan(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps, int32_t ncol, int32_t rows_dtype, int32_t form,
@@ -190,6 +243,17 @@ int mfcc_gated_scan(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps
   if (const int rc = check_grid(who, s, c, workspace)) return rc;
   const mfcc::ScanPtrs q{h0, nullptr, last, checkpoints, nullptr, (float2*)workspace};
   const size_t size = rows_dtype == MFCC_ROWS_F32 ? 4 : 2;
+  {
+    const int64_t ends = s.b.n_seq * ncol * (int64_t)sizeof(float);
+    const Bytes bx = bytes_of("x", x, s, size), bg = bytes_of("gate", gate, s, size), by = bytes_of("y", y, s, size), bh = bytes_of("h0", h0, ends),
+                bl = bytes_of("last", last, ends), bc = bytes_of("checkpoints", checkpoints, checkpoints_of(s, c) * (int64_t)sizeof(float)),
+                bw = bytes_of("workspace", workspace, workspace_of(s, c));
+    if (const int rc = check_apart(who, by, {bx, bg}, true)) return rc;
+    if (const int rc = check_apart(who, bl, {bx, bg, by, bh})) return rc;
+    if (const int rc = check_apart(who, by, {bh})) return rc;
+    if (const int rc = check_apart(who, bc, {bx, bg, by, bh, bl})) return rc;
+    if (const int rc = check_apart(who, bw, {bx, bg, by, bh, bl, bc})) return rc;
+  }
   const bool al = aligned(x, s, c.v, size) && aligned(gate, s, c.v, size) && aligned(y, s, c.v, size);
   c.w.near = near(x, c, s, size) && near(gate, c, s, size) && near(y, c, s, size);
   dispatch(rows_dtype, c.v, al, [&](auto zero, auto v, auto al) {
@@ -228,6 +292,17 @@ int mfcc_gated_scan_backward(const mfcc_layout* layout, int64_t n_seq, int64_t t
   if (const int rc = check_grid(who, s, c, workspace)) return rc;
   const mfcc::ScanPtrs q{nullptr, grad_last, nullptr, const_cast<float*>(checkpoints), grad_h0, (float2*)workspace};
   const size_t size = rows_dtype == MFCC_ROWS_F32 ? 4 : 2;
+  {
+    const int64_t ends = s.b.n_seq * ncol * (int64_t)sizeof(float);
+    const Bytes bx = bytes_of("x", x, s, size), bg = bytes_of("gate", gate, s, size), bd = bytes_of("grad_y", grad_y, s, size),
+                bl = bytes_of("grad_last", grad_last, ends), bc = bytes_of("checkpoints", checkpoints, checkpoints_of(s, c) * (int64_t)sizeof(float)),
+                gx = bytes_of("grad_x", grad_x, s, size), gg = bytes_of("grad_gate", grad_gate, s, size), gh = bytes_of("grad_h0", grad_h0, ends),
+                bw = bytes_of("workspace", workspace, workspace_of(s, c));
+    if (const int rc = check_apart(who, gx, {bx, bg, bd, bl, bc})) return rc;
+    if (const int rc = check_apart(who, gg, {bx, bg, bd, bl, bc, gx})) return rc;
+    if (const int rc = check_apart(who, gh, {bx, bg, bd, bl, bc, gx, gg})) return rc;
+    if (const int rc = check_apart(who, bw, {bx, bg, bd, bl, bc, gx, gg, gh})) return rc;
+  }
   const bool al = aligned(x, s, c.v, size) && aligned(gate, s, c.v, size) && aligned(grad_y, s, c.v, size) && aligned(grad_x, s, c.v, size) &&
             aligned(grad_gate, s, c.v, size);
   c.w.near = near(x, c, s, size) && near(gate, c, s, size) && near(grad_y, c, s, size) && near(grad_x, c, s, size) && near(grad_gate, c, s, size);
@@ -250,24 +325,33 @@ int mfcc_gated_scan_backward(const mfcc_layout* layout, int64_t n_seq, int64_t t
 int mfcc_gated_scan_step(int64_t n_seq, int32_t ncol, int32_t rows_dtype, int32_t form, const void* x, int64_t x_ld, const void* gate,
                          int64_t gate_ld, const float* state_in, float* state_out, void* y, int64_t y_ld, void* stream) {
   static const char who[] = "mfcc_gated_scan_step";
-  if (ncol < 1 || ncol > kMaxColumns || n_seq < 0 || n_seq > INT32_MAX || x_ld < 0 || gate_ld < 0) return fail(MFCC_ERR_INVALID, "%s: bad shape", who);
+  if (ncol < 1 || ncol > kMaxColumns || n_seq < 0 || n_seq > INT32_MAX || x_ld < 0 || gate_ld < 0 ||
+      std::max({x_ld, gate_ld, y_ld}) > kMaxStride)
+    return fail(MFCC_ERR_INVALID, "%s: bad shape", who);
   if (n_seq > 1 && y_ld < ncol) return fail(MFCC_ERR_INVALID, "%s: rows of y overlap", who);
   if (form != MFCC_SCAN_DECAY && form != MFCC_SCAN_SIGMOID) return fail(MFCC_ERR_INVALID, "%s: form=%d", who, form);
   if (n_seq == 0) return MFCC_OK;
   if (n_seq * ncol > kMaxThreads - 255) return fail(MFCC_ERR_UNSUPPORTED, "%s: too many values per call", who);
   if (!x || !gate || !state_in || !state_out || !y) return fail(MFCC_ERR_INVALID, "%s: null pointer", who);
+  if (rows_dtype < 0 || rows_dtype > MFCC_ROWS_F16) return bad_dtype(who, rows_dtype);
+  {
+    // a thread reads its element everywhere before it writes it: any of the arrays may be one and the same
+    const int64_t size = rows_dtype == MFCC_ROWS_F32 ? 4 : 2;
+    auto rows = [&](const char* name, const void* p, int64_t e, int64_t ld) { return Bytes{name, (const char*)p, ncol * e, n_seq > 1 ? ld * e : 0, 0, n_seq, 1}; };
+    const Bytes bx = rows("x", x, size, x_ld), bg = rows("gate", gate, size, gate_ld), by = rows("y", y, size, y_ld),
+                bi = rows("state_in", state_in, 4, ncol), bo = rows("state_out", state_out, 4, ncol);
+    if (const int rc = check_apart(who, by, {bx, bg, bi, bo}, true)) return rc;
+    if (const int rc = check_apart(who, bo, {bx, bg, bi}, true)) return rc;
+  }
   auto go = [&](auto zero) {
     using T = decltype(zero);
     auto k = form == MFCC_SCAN_SIGMOID ? mfcc::gated_scan_step_kernel<T, true> : mfcc::gated_scan_step_kernel<T, false>;
     hipLaunchKernelGGL(k, dim3(blocks_for(n_seq * ncol, 256)), dim3(256), 0, (hipStream_t)stream, n_seq, ncol, (const T*)x, x_ld,
                        (const T*)gate, gate_ld, state_in, state_out, (T*)y, y_ld);
   };
-  switch (rows_dtype) {
-    case MFCC_ROWS_F32: go(0.0f); break;
-    case MFCC_ROWS_BF16: go((mfcc::bf16)0.0f); break;
-    case MFCC_ROWS_F16: go((mfcc::f16)0.0f); break;
-    default: return bad_dtype(who, rows_dtype);
-  }
+  if (rows_dtype == MFCC_ROWS_F32) go(0.0f);
+  else if (rows_dtype == MFCC_ROWS_BF16) go((mfcc::bf16)0.0f);
+  else go((mfcc::f16)0.0f);
   HIP_TRY(hipGetLastError());
   return MFCC_OK;
 }
@@ -282,7 +366,6 @@ int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_ste
   if (!(eps >= 0.0 && eps <= 1e30)) return fail(MFCC_ERR_INVALID, "%s: eps=%g", who, eps);
   if (const int rc = check_rows(who, "x", x, s, false)) return rc;
   if (const int rc = check_rows(who, "y", y, s, true)) return rc;
-  if (state_in && state_in == state_out) return fail(MFCC_ERR_INVALID, "%s: state_out needs an array of its own", who);
   if (y_dtype < 0 || y_dtype > MFCC_ROWS_F16) return bad_dtype(who, y_dtype);
   if (s.b.n_seq == 0) return MFCC_OK;
   Grid c = grid_of(s);
@@ -292,6 +375,15 @@ int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_ste
     if (const int rc = check_grid(who, s, c, workspace)) return rc;
   }
   const size_t size = y_dtype == MFCC_ROWS_F32 ? 4 : 2;
+  {
+    const int64_t ends = s.b.n_seq * (1 + 2 * (int64_t)ncol) * (int64_t)sizeof(float);
+    const Bytes bx = bytes_of("x", x, s, 4), by = bytes_of("y", y, s, size), bi = bytes_of("state_in", state_in, ends),
+                bo = bytes_of("state_out", state_out, ends), bw = bytes_of("workspace", workspace, workspace_of(s, c));
+    if (const int rc = check_apart(who, by, {bx}, true)) return rc;
+    if (const int rc = check_apart(who, by, {bi})) return rc;
+    if (const int rc = check_apart(who, bo, {bx, by, bi})) return rc;
+    if (const int rc = check_apart(who, bw, {bx, by, bi, bo})) return rc;
+  }
   const bool al = aligned(x, s, c.v, 4) && aligned(y, s, c.v, size);
   c.w.near = near(x, c, s, 4) && near(y, c, s, size);
   mfcc::NormArgs a;
@@ -346,6 +438,11 @@ int mfcc_feature_dropout(const mfcc_layout* layout, int64_t n_seq, int64_t time_
   const mfcc::Dropout d{seed, step, step_device, (uint32_t)threshold, threshold < 65536 ? 65536.0f / (float)(65536 - threshold) : 0.0f};
   const size_t size = rows_dtype == MFCC_ROWS_F32 ? 4 : 2;
   const int64_t most = (int64_t)INT32_MAX * 8;
+  {
+    const Bytes by = bytes_of("y", y, s, size);
+    if (const int rc = check_apart(who, by, {bytes_of("x", x, s, size)}, true)) return rc;
+    if (const int rc = check_apart(who, by, {bytes_of("step_device", step_device, sizeof(int64_t))})) return rc;
+  }
   hipStream_t st = (hipStream_t)stream;
   // a batch without padding between its rows is one run of rows
   auto flat = [&](const mfcc_rows* r) {

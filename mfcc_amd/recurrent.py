@@ -9,7 +9,8 @@ with frame counts (``MFCC.forward``), or a padded ``[B, T, D]`` batch with lengt
 repeated batch shapes; required while a stream is being captured) or None: all rows are one sequence
 (2-D) or every sequence is full (3-D).  Lengths beyond T count as T, as ``pad_sequences`` reports
 them.  Rows behind the end of a padded sequence are not read; outputs hold 0 there.  Derivatives are those of
-backward passes: tensors that carry a forward-mode tangent are refused.
+backward passes: tensors that carry a forward-mode tangent are refused.  So are ``out`` and ``state_out``
+that overlap another tensor of the call, unless they are the very tensor that a call may work on in place.
 """
 from __future__ import annotations
 
@@ -212,7 +213,7 @@ def gated_scan(x, gate, frame_counts=None, h0=None, form="decay", reverse=False,
     float32 state behind the last row [n_seq, D] (``h0`` where a sequence is empty), which is the ``h0``
     of the next piece.  The state is float32 throughout.  Differentiable in x, gate and h0 (once): the
     backward pass computes the states again from float32 checkpoints instead of reading the rounded y.
-    ``out`` takes y when no gradient is asked for; it may be ``x``."""
+    ``out`` takes y when no gradient is asked for; it may be ``x`` or ``gate``."""
     _check(x, "x")
     _check(gate, "gate", like=x)
     _no_tangent(x, gate, h0, out)

@@ -43,3 +43,21 @@ def test_forward_mode_is_refused(M):
                 with mode(), pytest.raises(ValueError, match="tangent"):
                     call()
         assert torch.equal(M.gated_scan(x, g)[0], M.gated_scan(x, g)[0])    # tensors without one go on as ever
+
+
+def test_overlap_is_refused(M):
+    from mfcc_amd import _capi as capi
+    buf = torch.rand(2, 21, 8, device="cuda")
+    x, g = buf[:, :20], torch.rand(2, 20, 8, device="cuda")
+    st = torch.zeros(3, 17, device="cuda")
+    h = torch.zeros(3, 8, device="cuda")
+    for f in (lambda: M.gated_scan(x, g, out=buf[:, 1:]), lambda: M.gated_scan(g, x, out=buf[:, 1:]), lambda: M.running_norm(x, out=buf[:, 1:]),
+              lambda: M.running_norm(x, state=st[:2], state_out=st[1:]), lambda: M.running_norm(x, state=st[1:], state_out=st[:2]),
+              lambda: M.feature_dropout(x, 0.5, 1, out=buf[:, 1:]), lambda: M.gated_scan_step(g[0, :2], g[1, :2], h[:2], state_out=h[1:]),
+              lambda: M.gated_scan_step(buf[0, :2], g[1, :2], h[:2], out=buf[0, 1:3])):
+        with pytest.raises(capi.MfccError, match="overlaps"):
+            f()
+    wide = torch.rand(2, 20, 24, device="cuda")       # parts of the same rows do not
+    a, b, c = wide[..., :8], wide[..., 8:16], wide[..., 16:]
+    want = M.gated_scan(a, b)[0]
+    assert torch.equal(M.gated_scan(a, b, out=c)[0], want) and torch.equal(M.gated_scan(a, b, out=b)[0], want)
