@@ -299,6 +299,9 @@ typedef struct mfcc_rows {
  *   MFCC_SCAN_SIGMOID  h_t = a_t h_{t-1} + (1 - a_t) x_t,  a_t = 1 / (1 + exp(-gate_t))
  * y_t = h_t rounded to the type of the rows; last (float32 [n_seq, ncol], may be NULL) = the state behind the
  * last row, h0 for an empty sequence.  reverse = 1: t runs from the last row of a sequence to its first.
+ * Rows are composed: the product of the gates of 8 neighbouring rows is one float32 number (longer runs keep their exponent
+ * apart).  Where it underflows (all 8 below 2e-6) an infinite state before them becomes NaN instead of staying infinite; where it
+ * overflows (all 8 above 6e4) a state of 0 becomes NaN.
  * checkpoints: NULL, or mfcc_gated_scan_checkpoints() floats that receive states for the backward pass.
  * workspace: mfcc_sequence_workspace() bytes of device memory, 16-byte aligned, used by this call only (may be NULL
  * where that is 0).  y may be x or gate. */

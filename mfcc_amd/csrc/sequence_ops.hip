@@ -123,7 +123,7 @@ int64_t checkpoints_of(const Shape& s, const Grid& g) {
   const int64_t k = g.tile_rows, t = s.b.steps;
   return (t || !s.b.off ? s.b.n_seq * ((t + k - 1) / k) : s.rows / k + s.b.n_seq) * s.b.ncol;
 }
-int64_t workspace_of(const Shape& s, const Grid& g) { return g.w.pieces > 1 ? s.b.n_seq * g.w.pieces * s.b.ncol * (int64_t)sizeof(float2) : 0; }
+int64_t workspace_of(const Shape& s, const Grid& g) { return g.w.pieces > 1 ? s.b.n_seq * g.w.pieces * s.b.ncol * (int64_t)sizeof(mfcc::ScanMap) : 0; }
 
 int check_grid(const char* who, const Shape& s, const Grid& g, const void* workspace) {
   if (((int64_t)g.w.blocks + 7) / 8 * 8 * g.w.column_blocks > kMaxThreads / g.threads)
@@ -241,7 +241,7 @@ int mfcc_gated_scan(const mfcc_layout* layout, int64_t n_seq, int64_t time_steps
   if (s.b.n_seq == 0) return MFCC_OK;
   Grid c = grid_of(s);
   if (const int rc = check_grid(who, s, c, workspace)) return rc;
-  const mfcc::ScanPtrs q{h0, nullptr, last, checkpoints, nullptr, (float2*)workspace};
+  const mfcc::ScanPtrs q{h0, nullptr, last, checkpoints, nullptr, (mfcc::ScanMap*)workspace};
   const size_t size = rows_dtype == MFCC_ROWS_F32 ? 4 : 2;
   {
     const int64_t ends = s.b.n_seq * ncol * (int64_t)sizeof(float);
@@ -290,7 +290,7 @@ int mfcc_gated_scan_backward(const mfcc_layout* layout, int64_t n_seq, int64_t t
   if (s.b.n_seq == 0) return MFCC_OK;
   Grid c = grid_of(s);
   if (const int rc = check_grid(who, s, c, workspace)) return rc;
-  const mfcc::ScanPtrs q{nullptr, grad_last, nullptr, const_cast<float*>(checkpoints), grad_h0, (float2*)workspace};
+  const mfcc::ScanPtrs q{nullptr, grad_last, nullptr, const_cast<float*>(checkpoints), grad_h0, (mfcc::ScanMap*)workspace};
   const size_t size = rows_dtype == MFCC_ROWS_F32 ? 4 : 2;
   {
     const int64_t ends = s.b.n_seq * ncol * (int64_t)sizeof(float);

@@ -211,8 +211,10 @@ def gated_scan(x, gate, frame_counts=None, h0=None, form="decay", reverse=False,
     ``gate[D]`` is one gate for all rows); ``reverse`` runs each sequence from its last row to its first,
     the other half of a bidirectional layer.  Returns (y, last): y_t = h_t in the type of ``x``, and the
     float32 state behind the last row [n_seq, D] (``h0`` where a sequence is empty), which is the ``h0``
-    of the next piece.  The state is float32 throughout.  Differentiable in x, gate and h0 (once): the
-    backward pass computes the states again from float32 checkpoints instead of reading the rounded y.
+    of the next piece.  The state is float32 throughout; infinities and NaN stay in their sequence and column, from
+    their row on (an infinity may become NaN behind 8 rows whose gates multiply to less than 2^-149).  Differentiable
+    in x, gate and h0 (once): the backward pass computes the states again from float32 checkpoints instead of
+    reading the rounded y.
     ``out`` takes y when no gradient is asked for; it may be ``x`` or ``gate``."""
     _check(x, "x")
     _check(gate, "gate", like=x)

@@ -38,6 +38,11 @@ inline float __expf(float v) { return expf(v); }
 inline float sim_flushed(float v) { return fabsf(v) < std::numeric_limits<float>::min() ? copysignf(0.0f, v) : v; }
 #define __builtin_amdgcn_rcpf(v) (1.0f / sim_flushed(v))
 #define __builtin_amdgcn_rsqf(v) ((float)(1.0 / sqrt((double)sim_flushed(v))))
+inline float sim_frexp_mant(float v) { int e; return isfinite(v) ? frexpf(v, &e) : v; }
+inline int sim_frexp_exp(float v) { int e = 0; return isfinite(v) ? frexpf(v, &e), e : 0; }
+#define __builtin_amdgcn_frexp_mantf(v) sim_frexp_mant(v)
+#define __builtin_amdgcn_frexp_expf(v) sim_frexp_exp(v)
+#define __builtin_amdgcn_ldexpf(v, e) ldexpf(v, e)
 #define __builtin_amdgcn_readfirstlane(v) (v)
 
 typedef void* hipStream_t;

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_sequence_ops import M, U, check_norm, check_scan, host, norm_sequence  # noqa: F401
+from test_gpu_sequence_ops import HALF, TINY, M, U, check_norm, check_scan, host, make_gate, memory, norm_sequence, sequence  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +61,48 @@ def test_overlap_is_refused(M):
     a, b, c = wide[..., :8], wide[..., 8:16], wide[..., 16:]
     want = M.gated_scan(a, b)[0]
     assert torch.equal(M.gated_scan(a, b, out=c)[0], want) and torch.equal(M.gated_scan(a, b, out=b)[0], want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("form", ["decay", "sigmoid"])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_infinities_over_pieces(M, dtype, form, reverse):
+    """Long sequences: an infinity stays one over pieces whose products of gates vanish in 32 bits, forwards and backwards."""
+    n, d = 9000, 64
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    x, gy = (torch.randn(n, d, generator=gen, device="cuda").to(dtype) for _ in range(2))
+    g = make_gate(gen, (n, d), form, dtype)
+    g[g == 0] = 0.5
+    x[4000, 1], x[100, 2], x[8900, 3] = float("inf"), -float("inf"), float("inf")
+    gy[5000, 4], gy[8990, 5] = float("inf"), -float("inf")
+    h0, gl = (torch.randn(1, d, generator=gen, device="cuda") for _ in range(2))
+    h0[0, 6] = float("inf")
+    leaves = [t.requires_grad_(True) for t in (x, g, h0)]
+    y, last = M.gated_scan(x, g, [n], h0=h0, form=form, reverse=reverse)
+    dx, _, dh = torch.autograd.grad((y, last), leaves, (gy, gl))
+    with np.errstate(invalid="ignore"):
+        out, mag = sequence(host(x), host(g), host(h0)[0], form, reverse, host(gy), host(gl)[0])
+    mem = memory(host(g), form, n)
+    for got, ref, m, dt, what in ((y, out[0], mag[0], dtype, "y"), (last[0], out[1], mag[1], torch.float32, "last"), (dx, out[2], mag[2], dtype, "dx"),
+                                  (dh[0], out[4], mag[4], torch.float32, "dh0")):
+        got, fin = host(got), np.isfinite(ref)
+        assert (~fin).any() or reverse, what
+        assert np.array_equal(got[~fin], ref[~fin]), what
+        tol = 16 * U * (1 + mem) * m[fin] + HALF[dt] * np.abs(ref[fin]) + TINY[dt]
+        assert (np.abs(got[fin] - ref[fin]) <= tol).all(), what
+
+
+def test_products_of_gates_past_32_bits(M):
+    n, d = 9000, 64
+    x = torch.randn(n, d, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    g = torch.full((n, d), 0.9, device="cuda")
+    g[:6000, :4] = 1.1
+    x[:5900, 0] = 0              # nothing there to grow until shortly before the gates fall
+    x[:6000, 1], g[6000, 1] = 0, 0
+    g[:6001:500, 2] = 0          # 1.1 ** 500 = 5e20 in between
+    g[:6000, 3], x[:6000, 3] = -1.1, 0
+    y, last = M.gated_scan(x, g, [n])
+    out, mag = sequence(host(x), host(g), np.zeros(d), "decay", False)
+    assert np.isfinite(out[0]).all()
+    for got, ref, m in ((y, out[0], mag[0]), (last[0], out[1], mag[1])):
+        assert (np.abs(host(got) - ref) <= 16 * U * (1 + n) * m).all()

@@ -54,8 +54,8 @@ class Layout:
         self.sim.sim_layout_free(self.h)
 
 
-def workspace(sim, lay, d):
-    n = sim.mfcc_sequence_workspace(lay, 0, 0, d, capi.ROWS_F32)
+def workspace(sim, lay, d, steps=0):
+    n = sim.mfcc_sequence_workspace(lay, 1, steps, d, capi.ROWS_F32)
     assert n >= 0
     raw = np.full(n // 4 + 8, np.nan, np.float32)
     return raw[(-raw.ctypes.data % 16) // 4:]
@@ -115,3 +115,97 @@ def test_norm_last_column_block(sim, counts, d, last):
     div = division(sim, len(counts), max(counts), d)
     assert div[2] == last and (div[3] > 1) == (counts == [700]), div
     check_norm(sim, counts, d, seed=d, in_place=bool(d % 4 == 1))
+
+
+# --------------------------------------------------------------------------
+# the recurrence over sequences that are cut into pieces
+# --------------------------------------------------------------------------
+def run_scan(sim, x, g, h0=None, form=0, gy=None, glast=None):
+    """One packed float32 sequence: (y, last[, dx, dg, dh0])"""
+    n, d = x.shape
+    none = C.c_void_p(None)
+    head = none, 1, n, d, 0, form, 0
+    y, last = np.full_like(x, np.nan), np.full(d, np.nan, np.float32)
+    ws = workspace(sim, None, d, n)
+    ck = np.full(sim.mfcc_gated_scan_checkpoints(None, 1, n, d, 0), np.nan, np.float32)
+    assert sim.mfcc_gated_scan(*head, rows(x), rows(g), ptr(h0), rows(y), ptr(last), ptr(ck), ptr(ws), None) == 0
+    if gy is None:
+        return y, last
+    dx, dg, dh = np.full_like(x, np.nan), np.full_like(x, np.nan), np.full(d, np.nan, np.float32)
+    assert sim.mfcc_gated_scan_backward(*head, rows(x), rows(g), ptr(ck), rows(gy), ptr(glast), rows(dx), rows(dg), ptr(dh), ptr(ws), None) == 0
+    return y, last, dx, dg, dh
+
+
+def scan_definition(x, g, h0, form):
+    a = g if form == 0 else 1 / (1 + np.exp(-g))
+    b = x if form == 0 else x / (1 + np.exp(g))
+    h, m = h0.copy(), np.abs(h0)
+    y, mag, before = np.zeros_like(x), np.zeros_like(x), np.zeros_like(x)
+    for t in range(len(x)):
+        before[t] = h
+        h = a[t] * h + b[t]
+        m = np.abs(a[t]) * m + np.abs(b[t])
+        y[t], mag[t] = h, m
+    return y, mag, a, before
+
+
+def agree(got, ref, mag, length):
+    """Equal where not finite, otherwise within 16 u for each of `length` rows and for their products"""
+    fin = np.isfinite(ref)
+    assert np.array_equal(got[~fin], ref[~fin], equal_nan=True)
+    assert (np.abs(got[fin] - ref[fin]) <= 16 * U * (1 + length) * mag[fin] + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("form", [0, 1])
+def test_infinite_states_stay_infinite(sim, form):
+    """An infinity is carried over pieces whose products of gates vanish in 32 bits, forwards and backwards."""
+    n, d = 6000, 8
+    assert division(sim, 1, n, d)[3] > 1
+    rng = np.random.default_rng(form)
+    x, g, gy = (rng.standard_normal((n, d)).astype(np.float32) for _ in range(3))
+    if form == 0:
+        g = (1 / (1 + np.exp(-g))).astype(np.float32) * np.where(rng.random((n, d)) < 0.2, np.float32(-1), np.float32(1))
+    x[100, 1], x[2000, 2], x[5500, 3] = np.inf, -np.inf, np.inf
+    gy[5900, 4], gy[3000, 5] = np.inf, -np.inf
+    h0, gl = rng.standard_normal(d).astype(np.float32), rng.standard_normal(d).astype(np.float32)
+    h0[0], gl[6] = -np.inf, np.inf
+    y, last, dx, dg, dh = run_scan(sim, x, g, h0, form, gy, gl)
+    ref, mag, a, before = scan_definition(x.astype(np.float64), g.astype(np.float64), h0.astype(np.float64), form)
+    # gates of at most 1 / (1 + exp(-5)): a memory below 150 rows
+    agree(y, ref, mag, 150)
+    agree(last, ref[-1], mag[-1], 150)
+    assert np.isinf(ref[-1]).sum() == 4
+    e, em, finite = gl.astype(np.float64), np.abs(gl).astype(np.float64), np.isfinite(before) & np.isfinite(x)
+    na = np.ones_like(a) if form == 0 else 1 / (1 + np.exp(g.astype(np.float64)))
+    ex, exm, eg, egm = (np.zeros_like(ref) for _ in range(4))
+    for t in reversed(range(n)):
+        delta, dm = gy[t] + e, np.abs(gy[t]) + em
+        ex[t], exm[t] = na[t] * delta, na[t] * dm
+        with np.errstate(invalid="ignore"):
+            eg[t] = delta * before[t] if form == 0 else delta * a[t] * na[t] * (before[t] - x[t])
+            egm[t] = dm * np.maximum(mag[t - 1] if t else np.abs(h0), np.abs(x[t]))
+        e, em = a[t] * delta, np.abs(a[t]) * dm
+    agree(dx, ex, exm, 150)
+    agree(dh, e, em, 150)
+    agree(dg[finite], eg[finite], 2 * egm[finite], 300)
+
+
+def test_products_of_gates_past_32_bits(sim):
+    """Gates above 1 whose product overflows while the states stay finite: nothing there to grow, or a gate of 0 afterwards."""
+    n, d = 6000, 8
+    assert division(sim, 1, n, d)[3] > 1
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((n, d)).astype(np.float32)
+    g = np.full((n, d), 0.9, np.float32)
+    g[:4000, :4] = 1.1           # 1.1 ** 1536, a piece: 4e63
+    x[:3900, 0] = 0              # rows of 0 until shortly before they end
+    x[:4000, 1], g[4000, 1] = 0, 0
+    g[:4001:500, 2] = 0          # 1.1 ** 500 = 5e20 in between
+    g[:4000, 3], x[:4000, 3] = -1.1, 0
+    h0 = np.zeros(d, np.float32)
+    h0[4:] = 1e30
+    y, last = run_scan(sim, x, g, h0)
+    ref, mag, _, _ = scan_definition(x.astype(np.float64), g.astype(np.float64), h0.astype(np.float64), 0)
+    assert np.isfinite(ref).all() and np.abs(ref).max() < 3e38
+    agree(y, ref, mag, n)
+    agree(last, ref[-1], mag[-1], n)
