@@ -416,8 +416,8 @@ int mfcc_running_norm(const mfcc_layout* layout, int64_t n_seq, int64_t time_ste
       hipLaunchKernelGGL((mfcc::running_norm_pieces_kernel<v(), al()>), c.blocks, dim3(c.threads), 0, (hipStream_t)stream, s.b, c.w, rows_of<const float>(x, s), a);
     const int slots = c.w.seqs * c.w.per;
     const size_t shared = 2 * slots * ((1 + mfcc::kSlotRows / 4) * sizeof(float4) + v() * c.w.cb * sizeof(float2));
-    hipLaunchKernelGGL((mfcc::running_norm_kernel<T, v(), al()>), c.blocks, dim3(c.threads), shared, (hipStream_t)stream, s.b, c.w,
-                       rows_of<const float>(x, s), rows_of<T>(y, s), a);
+    auto k = a.eps < 0x1p-126f && !center_only ? mfcc::running_norm_kernel<T, v(), al(), true> : mfcc::running_norm_kernel<T, v(), al(), false>;
+    hipLaunchKernelGGL(k, c.blocks, dim3(c.threads), shared, (hipStream_t)stream, s.b, c.w, rows_of<const float>(x, s), rows_of<T>(y, s), a);
   });
   HIP_TRY(hipGetLastError());
   return MFCC_OK;

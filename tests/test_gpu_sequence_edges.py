@@ -106,3 +106,17 @@ def test_products_of_gates_past_32_bits(M):
     assert np.isfinite(out[0]).all()
     for got, ref, m in ((y, out[0], mag[0]), (last[0], out[1], mag[1])):
         assert (np.abs(host(got) - ref) <= 16 * U * (1 + n) * m).all()
+
+
+@pytest.mark.parametrize("eps", [0.0, 2.0 ** -149, 2.0 ** -127])
+def test_norm_of_subnormal_variances(M, eps):
+    """Variances around the smallest normal number without an eps that covers them."""
+    from test_sequence_kernels_cpu import norm_definition, small_variance_tolerance, small_variances
+    rng, n, d, decay = np.random.default_rng(5), 300, 24, 0.9
+    x = small_variances(rng, n, d)
+    y = M.running_norm(torch.from_numpy(x).cuda(), decay=decay, eps=eps)[0]
+    with np.errstate(invalid="ignore"):
+        ref, fin, _ = norm_definition(x.astype(np.float64), decay, np.zeros(1 + 2 * d), eps)
+    tol, known = small_variance_tolerance(x.astype(np.float64), ref, decay, fin)
+    known[0] = False
+    assert known.mean() > 0.5 and (np.abs(host(y) - ref)[known] <= tol[known] + 32 * U * 8).all()   # means of values below 8 sigma

@@ -209,3 +209,39 @@ def test_products_of_gates_past_32_bits(sim):
     assert np.isfinite(ref).all() and np.abs(ref).max() < 3e38
     agree(y, ref, mag, n)
     agree(last, ref[-1], mag[-1], n)
+
+
+# --------------------------------------------------------------------------
+# values at the ends of the range of the normalisation
+# --------------------------------------------------------------------------
+def small_variances(rng, n, d):
+    """Rows around 0 whose variances lie from 2^-140 to 2^-120, where the smallest normal number is 2^-126"""
+    return (rng.standard_normal((n, d)) * 2.0 ** rng.uniform(-70, -60, d)).astype(np.float32)
+
+
+def small_variance_tolerance(x, ref, decay, fin):
+    """A subnormal sum of squares is off by half a step, 2^-150, for each of its two roundings a row, all of which decay like the rows:
+    2^-149 / (1 - decay) in all, relative to the sum s halved by the root; the 32 u of the other roundings on top."""
+    s = np.zeros(x.shape[1])
+    rel = np.zeros_like(x)
+    m, w = np.zeros(x.shape[1]), 0.0
+    for t in range(len(x)):
+        w = decay * w + 1
+        off = x[t] - m
+        m = m + off / w
+        s = decay * s + off * (x[t] - m)
+        rel[t] = 2.0 ** -149 / (1 - decay) / np.maximum(s, 1e-300)
+    return np.abs(ref) * (rel + 64 * U), rel < 0.1
+
+
+@pytest.mark.parametrize("eps", [0.0, 2.0 ** -149, 2.0 ** -127])
+def test_norm_of_subnormal_variances(sim, eps):
+    rng, n, d, decay = np.random.default_rng(5), 300, 24, 0.9
+    x = small_variances(rng, n, d)
+    y = np.full_like(x, np.nan)
+    assert sim.mfcc_running_norm(None, 1, n, d, decay, eps, 0, rows(x), None, rows(y), 0, None, None, None) == 0
+    with np.errstate(invalid="ignore"):
+        ref, fin, _ = norm_definition(x.astype(np.float64), decay, np.zeros(1 + 2 * d), eps)
+    tol, known = small_variance_tolerance(x.astype(np.float64), ref, decay, fin)
+    known[0] = False             # 0 / sqrt(eps) of the first row
+    assert known.mean() > 0.5 and (np.abs(y - ref)[known] <= tol[known] + 32 * U * 8).all()   # means of values below 8 sigma
