@@ -772,7 +772,12 @@ __global__ void __launch_bounds__(kSeqThreads, 4) running_norm_kernel(const Batc
   if (t.on && a.state_in) {
     weight = a.state_in[state];
 #pragma unroll
-    for (int v = 0; v < V; ++v) mean[v] = a.state_in[state + 1 + t.col + v], square[v] = a.state_in[state + 1 + b.ncol + t.col + v];
+    for (int v = 0; v < V; ++v) {
+      // beside a weight of 0 the first row is the mean, whatever the state's was: a step from there would leave a rounding of the way between
+      // them, of either sign, where s has the product with that way added
+      mean[v] = weight < 0x1p-22 ? 0.0 : a.state_in[state + 1 + t.col + v];
+      square[v] = a.state_in[state + 1 + b.ncol + t.col + v];
+    }
   }
 
   auto work = [&](auto full, const Pack<float, V>(&in)[R], int tile) {

@@ -120,3 +120,20 @@ def test_norm_of_subnormal_variances(M, eps):
     tol, known = small_variance_tolerance(x.astype(np.float64), ref, decay, fin)
     known[0] = False
     assert known.mean() > 0.5 and (np.abs(host(y) - ref)[known] <= tol[known] + 32 * U * 8).all()   # means of values below 8 sigma
+
+
+def test_norm_from_a_state_without_weight(M):
+    """A prior of weight 0 is no prior, wherever its means are: as a state, over pieces, and in live streams."""
+    rng = np.random.default_rng(7)
+    for n in (1, 5, 40, 9000):
+        x = torch.from_numpy((rng.standard_normal((n, 39)) * 3 + 7).astype(np.float32)).cuda()
+        st = torch.zeros(1, 79, device="cuda")
+        st[:, 1:40] = torch.from_numpy(rng.standard_normal(39) * 1000)
+        y, end = M.running_norm(x, state=st)
+        want, fin = M.running_norm(x)
+        assert torch.equal(y, want) and torch.equal(end, fin)
+    sums = torch.cat([torch.tensor([50.0]), torch.full((39,), 5e4), torch.full((39,), 6e7)]).double().cuda()     # means of 1000
+    audio = torch.from_numpy((rng.standard_normal((2, 8000)) * 3000).astype(np.int16)).cuda()
+    a = M.StreamingMFCC("self5", n_streams=2, max_chunk=8000, running_norm=0.98)
+    b = M.StreamingMFCC("self5", n_streams=2, max_chunk=8000, running_norm=0.98, norm_state=M.running_norm_state(sums, 0.0))
+    assert torch.equal(a.push(audio), b.push(audio)) and torch.equal(a.flush(), b.flush())

@@ -245,3 +245,22 @@ def test_norm_of_subnormal_variances(sim, eps):
     tol, known = small_variance_tolerance(x.astype(np.float64), ref, decay, fin)
     known[0] = False             # 0 / sqrt(eps) of the first row
     assert known.mean() > 0.5 and (np.abs(y - ref)[known] <= tol[known] + 32 * U * 8).all()   # means of values below 8 sigma
+
+
+@pytest.mark.parametrize("w0", [0.0, 2.0 ** -30, 2.0 ** -10])
+def test_norm_from_a_state_without_weight(sim, w0):
+    """Means far away that carry no weight leave nothing behind."""
+    rng, d = np.random.default_rng(6), 40
+    for n in (1, 5, 40, 3000):
+        x = (rng.standard_normal((n, d)) * 3 + 7).astype(np.float32)
+        st = np.concatenate([[w0], rng.standard_normal(d) * 1000, np.zeros(d)]).astype(np.float32)
+        y, end = np.full_like(x, np.nan), np.full_like(st, np.nan)
+        ws = workspace(sim, None, d, n)
+        assert sim.mfcc_running_norm(None, 1, n, d, 0.9, 1e-5, 0, rows(x), ptr(st), rows(y), 0, ptr(end), ptr(ws), None) == 0
+        counted = st.astype(np.float64) if w0 > 2.0 ** -22 else np.zeros(1 + 2 * d)
+        ref, fin, sig = norm_definition(x.astype(np.float64), 0.9, counted, 1e-5)
+        big = max(np.abs(x).max(), np.abs(counted[1:1 + d]).max())
+        assert (np.abs(y - ref) <= 32 * U * (big / sig + np.abs(ref) * (1 + big / sig)) + U * np.abs(ref)).all()
+        assert (np.abs(end[1:1 + d] - fin[1:1 + d]) <= 32 * U * big).all()
+        if w0 < 2.0 ** -22:
+            assert not y[0].any()
