@@ -18,3 +18,12 @@ def test_tangents_are_seen():
         with torch.inference_mode():     # nothing is differentiated there, in any mode
             recurrent._no_tangent(dual)
     recurrent._no_tangent(x)
+
+
+def test_state_from_sums_of_no_rows():
+    """An accumulator that has seen nothing is no prior, whatever weight it is given."""
+    for weight in (0.0, 50.0):
+        assert recurrent.running_norm_state(torch.zeros(7, dtype=torch.float64), weight, 2).tolist() == [[0.0] * 7] * 2
+    sums = torch.tensor([4.0, 8.0, -4.0, 20.0, 4.0], dtype=torch.float64)
+    assert recurrent.running_norm_state(sums, 10.0).tolist() == [[10.0, 2.0, -1.0, 10.0, 0.0]]
+    assert recurrent.running_norm_state(sums, 0.0).tolist() == [[0.0, 2.0, -1.0, 0.0, 0.0]]
