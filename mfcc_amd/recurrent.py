@@ -315,11 +315,12 @@ def running_norm(feats, frame_counts=None, decay=0.995, state=None, eps=1e-5, ce
 
 def running_norm_state(sums, weight, n_seq=1):
     """State of :func:`running_norm` that starts from corpus statistics: ``sums`` = the float64 (n, sum x,
-    sum x^2) of ``cmvn_accumulate``, counted as ``weight`` rows -> float32 [n_seq, 1 + 2 D].  Sums of no rows give the state 0, whatever the weight."""
+    sum x^2) of ``cmvn_accumulate``, counted as ``weight`` rows -> float32 [n_seq, 1 + 2 D].  Sums of no rows give the state 0,
+    whatever the weight."""
     if sums.dim() != 1 or sums.numel() < 3 or sums.numel() % 2 == 0 or sums.dtype != torch.float64:
         raise ValueError("sums must be a float64 vector of 1 + 2*D elements")
-    if not weight >= 0:
-        raise ValueError("weight must not be negative")
+    if not 0 <= weight < float("inf"):
+        raise ValueError("weight must be finite and not negative")
     d = (sums.numel() - 1) // 2
     some = sums[:1] > 0
     n = torch.where(some, sums[:1], 1.0)

@@ -27,3 +27,6 @@ def test_state_from_sums_of_no_rows():
     sums = torch.tensor([4.0, 8.0, -4.0, 20.0, 4.0], dtype=torch.float64)
     assert recurrent.running_norm_state(sums, 10.0).tolist() == [[10.0, 2.0, -1.0, 10.0, 0.0]]
     assert recurrent.running_norm_state(sums, 0.0).tolist() == [[0.0, 2.0, -1.0, 0.0, 0.0]]
+    for bad in (-1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            recurrent.running_norm_state(sums, bad)
