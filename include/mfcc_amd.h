@@ -329,8 +329,10 @@ int mfcc_gated_scan_step(int64_t n_seq, int32_t ncol, int32_t rows_dtype, int32_
  * (float32 [n_seq, 1 + 2 ncol]: weight, means, weighted sums of squared deviations; NULL = all 0)
  *   w_t = decay w_{t-1} + 1,  m_t = m_{t-1} + (x_t - m_{t-1}) / w_t,  s_t = decay s_{t-1} + (x_t - m_{t-1})(x_t - m_t)
  *   y_t = (x_t - m_t) / sqrt(s_t / w_t + eps)            (center_only = 1: y_t = x_t - m_t)
- * A w_0 below 2^-22 counts as 0, so that m_1 = x_1.  0 < decay <= 1 (1: cumulative statistics; exact up to 2^24 rows),
- * eps >= 0 (squares of deviations are summed in float32: below 2^-126 they keep fewer digits).  The streaming counterpart
+ * A w_0 below 2^-22 counts as 0, so that m_1 = x_1.  0 < decay <= 1 (1: cumulative statistics).  The state is
+ * float32: w counts rows exactly up to 2^24, m and s are rounded at the end of every call (inside one the means are carried in 64 bits),
+ * so that a step (x_t - m) / w below half a unit in m's last place is lost between calls: calls of few rows stop following after
+ * some million rows at decay = 1.  eps >= 0 (squares of deviations are summed in float32: below 2^-126 they keep fewer digits).  The streaming counterpart
  * of the corpus constants (x + mm) .* vv (anal_recog_nn_liste.m:180) and of the per-utterance (x - mean) / std
  * (inference_ctc_eri_05.py:291), which need the whole corpus or utterance.  x is float32; y has y_dtype and may be x
  * when that is float32.  state_out (may be NULL): the state behind the last row, in an array of its own. */

@@ -275,9 +275,10 @@ def running_norm(feats, frame_counts=None, decay=0.995, state=None, eps=1e-5, ce
         y_t = (x_t - m_t) / sqrt(s_t / w_t + eps)          (``center_only``: y_t = x_t - m_t)
 
     so it needs neither the whole utterance (``utterance_scalar_norm``) nor a corpus (``cmvn_apply``) and serves
-    live streams.  ``decay=1`` gives cumulative statistics (up to 2^24 rows).  ``state``: float32
-    [n_seq, 1 + 2 D] = (w, m, s) before the first row, default 0; :func:`running_norm_state` makes one from
-    corpus sums.  Returns (y, state behind the last row).  ``dtype``: type of y, float32 (default), bfloat16
+    live streams.  ``decay=1`` gives cumulative statistics.  ``state``: float32 [n_seq, 1 + 2 D] = (w, m, s) before
+    the first row, default 0: w counts rows exactly up to 2^24, m and s are rounded once a call, so that calls of few
+    rows (live streams) stop following after some million rows at ``decay=1``.  :func:`running_norm_state` makes a
+    state from corpus sums.  Returns (y, state behind the last row).  ``dtype``: type of y, float32 (default), bfloat16
     or float16; ``out`` may be ``feats`` when that is float32; ``state_out`` is an array of its own.  Feature rows
     have no gradient here: an input that requires one is refused."""
     _check(feats, "feats", dtypes=(torch.float32,))
