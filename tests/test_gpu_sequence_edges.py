@@ -137,3 +137,50 @@ def test_norm_from_a_state_without_weight(M):
     a = M.StreamingMFCC("self5", n_streams=2, max_chunk=8000, running_norm=0.98)
     b = M.StreamingMFCC("self5", n_streams=2, max_chunk=8000, running_norm=0.98, norm_state=M.running_norm_state(sums, 0.0))
     assert torch.equal(a.push(audio), b.push(audio)) and torch.equal(a.flush(), b.flush())
+
+
+def time_major(*shape, dtype=torch.float32):
+    """[B, T, D] whose memory runs over the sequences first"""
+    b, t, d = shape
+    return torch.empty(t, b, d, dtype=dtype, device="cuda").transpose(0, 1)
+
+
+@pytest.mark.parametrize("d", [39, 40, 257])
+@pytest.mark.parametrize("counts", [None, [30, 0, 17, 90, 5]])
+def test_orders_of_rows(M, d, counts):
+    """Inputs and outputs in time-major memory and between other columns give the bits of rows one after the other."""
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    x, g, gy = (torch.randn(5, 70, d, generator=gen, device="cuda") for _ in range(3))
+    xt, gt, gyt = (time_major(5, 70, d).copy_(t) for t in (x, g, gy))
+    wide = torch.full((5, 70, d + 9), 7.0, device="cuda")
+
+    def places(dtype):
+        yield time_major(5, 70, d, dtype=dtype)
+        w = wide.to(dtype)
+        yield w[..., 3:3 + d]
+        assert (w[..., :3] == 7).all() and (w[..., 3 + d:] == 7).all()
+
+    for dtype in (torch.float32, torch.bfloat16):
+        z, s = M.running_norm(x, counts, dtype=dtype)
+        for out in places(dtype):
+            z2, s2 = M.running_norm(xt, counts, out=out)
+            assert z2 is out and torch.equal(z2, z) and torch.equal(s2, s)
+        xd = x.to(dtype)
+        for per in ("element", "frame", "sequence"):
+            want = M.feature_dropout(xd, 0.4, 5, per=per, frame_counts=counts)
+            for out in places(dtype):
+                assert torch.equal(M.feature_dropout(xt.to(dtype), 0.4, 5, per=per, frame_counts=counts, out=out), want)
+                assert torch.equal(M.feature_dropout(out.copy_(xd), 0.4, 5, per=per, frame_counts=counts, out=out), want)
+        gd = g.to(dtype)
+        want, last = M.gated_scan(xd, gd, counts, form="sigmoid", reverse=True)
+        for out in places(dtype):
+            assert torch.equal(M.gated_scan(xt.to(dtype), gt.to(dtype), counts, form="sigmoid", reverse=True, out=out)[0], want)
+    grads = []
+    for a, b, c in ((x, g, gy), (xt, gt, gyt)):
+        a, b = a.detach().requires_grad_(True), b.detach().requires_grad_(True)
+        y, last = M.gated_scan(a, b, counts, form="sigmoid")
+        grads.append((y.detach(), last.detach()) + torch.autograd.grad(y, (a, b), c))
+    assert all(torch.equal(p, q) for p, q in zip(*grads))
+    xr = xt.detach().requires_grad_(True)
+    (dx,) = torch.autograd.grad(M.feature_dropout(xr, 0.4, 5, per="sequence"), xr, gyt)
+    assert torch.equal(dx, M.feature_dropout(gy, 0.4, 5, per="sequence"))
