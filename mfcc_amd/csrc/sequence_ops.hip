@@ -58,8 +58,9 @@ int check_rows(const char* who, const char* name, const mfcc_rows* r, const Shap
 
 // Where workgroups of one sequence are fewer than the compute units, sequences of many tiles are cut into pieces, and others spread over
 // narrower column blocks.  Measured with 512 columns of bfloat16, forward (training step): one sequence of 512 rows (8 tiles)
-// 11.1 (31.6) us whole, 12.8 (27.8) in pieces of 2 tiles; of 1024 rows 18.8 (56.6) and 13.3 (29.0), of 8192 rows 124 (396) and
-// 17.1 (38.8).  32 sequences of up to 700 rows (11 tiles, 4 pieces would fill the card) 18.9 us whole, 28 in pieces.
+// 11.1 (31.6) us whole, 12.8 (27.8) in pieces of 2 tiles; of 1024 rows 18.8 (56.6) and 13.8 (29.3), of 8192 rows 124 (396) and
+// 18.3 (38.5).  32 sequences of up to 700 rows (11 tiles, 4 pieces would fill the card) 18.9 us whole, 28 in pieces.
+// All sequences get the same number of pieces: one long one among many short ones gets few, and from 256 workgroups on none.
 constexpr int64_t kFewBlocks = 256, kManyTiles = 10, kManyPieces = 5, kTargetBlocks = 512, kPieceTiles = 2;
 
 // Workgroups of half the threads for the normalisation where there are many: half the slots to join a tile (10000 sequences of
