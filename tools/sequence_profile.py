@@ -11,6 +11,7 @@ import collections
 import csv
 import glob
 import os
+import re
 import sys
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -35,12 +36,13 @@ def rows(folder, kind):
     out = []
     for f in glob.glob(os.path.join(folder, "**", f"*{kind}.csv"), recursive=True):
         with open(f) as h:
-            out += [r for r in csv.DictReader(h) if "mfcc::" in r["Kernel_Name"]]
+            out += [r for r in csv.DictReader(h) if "mfcc" in r["Kernel_Name"]]
     return sorted(out, key=lambda r: int(r["Start_Timestamp"]))
 
 
 def name(r):
-    return r["Kernel_Name"].split("mfcc::")[1].split("(")[0]
+    """The kernel, and the types in its name that the profiler leaves mangled or garbles where they are 16 bits wide"""
+    return re.search(r"[a-z][a-z_]*_kernel", r["Kernel_Name"]).group(), r["Kernel_Name"]
 
 
 def median(v):
@@ -56,7 +58,7 @@ def table(trace, counters=None):
     for r in rows(counters, "counter_collection") if counters else []:
         found[name(r), int(r["Grid_Size"])][r["Counter_Name"]].append(float(r["Counter_Value"]))
     for key, v in times.items():
-        line = f"{key[0]:58s} threads {key[1]:9d}  launches {len(v):3d}  median {median(v):7.1f} us  min {min(v):7.1f}"
+        line = f"{key[0][0]:26s} threads {key[1]:9d}  launches {len(v):3d}  median {median(v):7.1f} us  min {min(v):7.1f}"
         c = {n: median(w) for n, w in found[key].items()}
         if c:
             line += f"  vector issue {c['SQ_INSTS_VALU'] / 1024 * 4 / (c['GRBM_GUI_ACTIVE'] / 8):.2f}"
